@@ -28,7 +28,8 @@ extern "C" {
 #endif
 
 /* raised when an entry point changes or goes; a library from before one was added has the same
- * version and lacks the symbol (since version 1: xgen_fp8_quantize_tensor) */
+ * version and lacks the symbol (since version 1: xgen_fp8_quantize_tensor, xgen_residual_norm, xgen_route,
+ * xgen_route_workspace_bytes, xgen_grouped_matmul, xgen_expert_combine) */
 #define XGEN_ABI_VERSION 1
 
 /* status codes */
@@ -52,7 +53,8 @@ extern "C" {
 /* widest row (head_dim) of the FP8 wire codec (the reference takes any multiple of 4) */
 #define XGEN_WIRE_MAX_WIDTH 1024
 
-/* normalisation kinds for xgen_norm_affine_quant */
+/* normalisation kinds for xgen_norm_affine_quant and xgen_residual_norm */
+#define XGEN_NORM_NONE (-1) /* xgen_residual_norm: the branch as it is */
 #define XGEN_NORM_LAYER 0 /* (x - mean) * rsqrt(var + eps), biased variance */
 #define XGEN_NORM_RMS 1   /* x * rsqrt(mean(x^2) + eps) */
 /* OR-ed into norm_kind: scale_table holds bf16(1 + scale) (xgen_adaln_one_plus) */
@@ -61,6 +63,12 @@ extern "C" {
 /* GEMM epilogue activations */
 #define XGEN_ACT_NONE 0
 #define XGEN_ACT_GELU_TANH 1 /* out = bf16(gelu_tanh(bf16(linear))) */
+
+/* expert router: scoring functions, and the largest expert and choice counts */
+#define XGEN_ROUTE_SOFTMAX 0
+#define XGEN_ROUTE_SIGMOID 1
+#define XGEN_ROUTE_MAX_EXPERTS 512
+#define XGEN_ROUTE_MAX_CHOICES 32
 
 /* Largest row width of the fused norm kernel (the reference limit,
  * x_base/x_base/operator/npu_fusion/capabilities.py:7, is 6144). */
@@ -447,6 +455,90 @@ int xgen_fp8_wire_encode_masked(int in_dtype, int streams, const void *q, const 
 int xgen_fp8_wire_decode_strided(int out_dtype, int streams, const void *wire, int64_t peers, int64_t seq,
                                  int64_t batch, int64_t heads, int64_t width, const int64_t *dst_strides,
                                  int64_t valid_seq, void *q, void *k, void *v, hipStream_t stream);
+
+/*
+ * The norms behind and in front of a block's branch, with its gate, its residual scale, the AdaLN-table
+ * modulation and the next projection's per-row quantization in one pass (no counterpart in the reference,
+ * whose blocks norm in front only: xgen_gate_residual followed by xgen_norm_affine_quant is its form):
+ *   stream = residual_scale * x + gate_table[g] * (norm_b(branch) * branch_weight),  g = indices[s]
+ *   h      = norm(stream) * norm_weight * (1 + scale_table[g]) + shift_table[g]
+ *   out    = bf16(h), or its rows quantized as xgen_quantize_rows does (from h unrounded)
+ * in fp32 throughout: stream_out = bf16(stream), and the rows, are the only roundings.
+ * x, branch: BF16 [batch, seq, width], strides in elements, last stride 1.  branch_norm: XGEN_NORM_NONE
+ * (the branch as it is, no branch_weight), _LAYER or _RMS; norm_kind _LAYER or _RMS.  Weights: NULL or
+ * [width], both of norm_weight_dtype (BF16/F32; NONE when both are NULL).  gate_table, and scale_table with
+ * shift_table: NULL or BF16 [table_rows, width]; indices int64 [seq] if any is given.  stream_out BF16,
+ * out (out_dtype BF16, E4M3 or I8): [batch, seq, width] contiguous; token_scale float32 [batch * seq]
+ * (ignored for BF16).  An index outside the tables makes what its row takes from them NaN: the stream
+ * if there is a gate, the rows in either case (quantized: NaN bytes or zeros, and a NaN scale).
+ * width <= XGEN_NORM_MAX_WIDTH; width and strides multiples of 8, buffers 16-byte aligned.
+ */
+int xgen_residual_norm(const void *x, int64_t x_stride_batch, int64_t x_stride_seq, const void *branch,
+                       int64_t br_stride_batch, int64_t br_stride_seq, int64_t batch, int64_t seq, int64_t width,
+                       int branch_norm, const void *branch_weight, int norm_kind, const void *norm_weight,
+                       int norm_weight_dtype, float residual_scale, float eps, const void *gate_table,
+                       int64_t gate_row_stride, const void *scale_table, int64_t scale_row_stride,
+                       const void *shift_table, int64_t shift_row_stride, int64_t table_rows,
+                       const int64_t *indices, void *stream_out, int out_dtype, void *out, float *token_scale,
+                       hipStream_t stream);
+
+/*
+ * Expert router: the k experts of every token, their weights, and the grouping of the (token, choice)
+ * pairs by expert that xgen_grouped_matmul and xgen_expert_combine take (no counterpart in the reference).
+ * logits: [tokens, experts] of in_dtype (BF16/F16/F32), rows ld elements apart.  A token's choices are the k
+ * largest of float(logit) + bias[e] (bias float32 [experts] or NULL; one fp32 addition), in descending
+ * order, ties to the lowest expert; -inf and NaN are never taken.  weights float32 [tokens, k]: of the
+ * logits without bias, softmax over all experts or sigmoid, divided by their sum over the taken experts if
+ * renormalize.  chosen int32 [tokens, k]: the experts.  Where fewer than k can be taken, chosen is -1 and
+ * the weight 0.  A NaN logit makes its token's weights NaN.
+ * Pairs of the experts [first_expert, first_expert + local_experts) are ordered by (expert, token,
+ * choice): ends int32 [local_experts] the pairs up to each one's last; rows int32 [tokens * k] the token
+ * of each pair, -1 behind the last; slots int32 [tokens, k] the place of each pair, -1 without one.
+ * The same on every run.  workspace: xgen_route_workspace_bytes(tokens, local_experts) bytes, 4-byte
+ * aligned.  experts <= XGEN_ROUTE_MAX_EXPERTS, k <= min(experts, XGEN_ROUTE_MAX_CHOICES), tokens >= 1,
+ * tokens * k < 2^31.
+ */
+size_t xgen_route_workspace_bytes(int64_t tokens, int64_t local_experts);
+int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t tokens, int64_t experts, int64_t k,
+               const float *bias, int scoring, int renormalize, int64_t first_expert, int64_t local_experts,
+               float *weights, int32_t *chosen, int32_t *ends, int32_t *rows, int32_t *slots, void *workspace,
+               size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * W8A8 products over ragged groups of rows, each with a weight of its own: the experts of a feed-forward,
+ * or the text and video rows of a dual-stream block (one xgen_scaled_mm_fp8 / _fp8_exact /
+ * xgen_quant_matmul_int8 call per group computes the same bits; no counterpart in the reference).
+ *   out[m, n] = out_dtype(acc * (a_scale[r] * w_scale[e, n]) + bias[e, n]),  acc = sum_k a[r, k] * w[e, n, k]
+ * (with XGEN_ACT_GELU_TANH out_dtype(gelu_tanh(.)) of it) for row m of group e, r = rows[m], or m if rows is
+ * NULL.  ends int32 [groups], on the device: group e is rows [ends[e - 1], ends[e]) (from 0); values are
+ * taken within [0, M], a group whose end lies before its begin is empty.  Output rows behind the last
+ * group's end are zeros.  a: [a_rows, K] of in_dtype (E4M3 or I8; exact: E4M3 products summed as
+ * xgen_scaled_mm_fp8_exact); rows int32 [M] or NULL (a_rows = M); a row index outside [0, a_rows) gives a NaN
+ * row.  w: [groups, N, K], rows ldw and groups w_group_stride elements apart.  a_scale_stride 0 or 1
+ * (one scale, or a_rows); w_scale_stride 0 ([groups]) or 1 ([groups, N]).  bias: NULL or [groups, N].
+ * out [M, N], rows ldo apart.  K, N multiples of 16, rows 16-byte aligned; one group's weight below
+ * 2 GiB, and with rows the activation too; groups <= XGEN_ROUTE_MAX_EXPERTS.
+ */
+int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64_t lda, int64_t a_rows, const void *w,
+                        int64_t ldw, int64_t w_group_stride, int64_t M, int64_t N, int64_t K, int64_t groups,
+                        const int32_t *ends, const int32_t *rows, const float *a_scale, int64_t a_scale_stride,
+                        const float *w_scale, int64_t w_scale_stride, const void *bias, int bias_dtype,
+                        int activation, void *out, int out_dtype, int64_t ldo, hipStream_t stream);
+
+/*
+ * Weighted sum of each token's expert rows, with the gated residual behind it (no counterpart in the
+ * reference; xgen_gate_residual is the gated residual alone):
+ *   out[t] = dtype(residual[t] + gate_table[indices[t % seq]] * sum_j weights[t, j] * y[slots[t, j]])
+ * summed in fp32 in the order of j, rounded once.  y: [y_rows, width] of dtype (BF16/F16), rows ldy apart;
+ * weights float32, slots int32, both [tokens, k]; a negative slot adds nothing, one at or past y_rows
+ * makes its row NaN.  residual: NULL or [tokens, width] of dtype; gate_table: NULL or [gate_rows, width]
+ * of dtype with indices int64 [seq], tokens a multiple of seq (an index outside: a NaN row).  out [tokens, width]
+ * contiguous.  width and strides multiples of 8, buffers 16-byte aligned.
+ */
+int xgen_expert_combine(int dtype, const void *y, int64_t ldy, int64_t y_rows, const float *weights,
+                        const int32_t *slots, int64_t tokens, int64_t k, int64_t width, const void *residual,
+                        int64_t ld_residual, const void *gate_table, int64_t gate_row_stride, int64_t gate_rows,
+                        const int64_t *indices, int64_t seq, void *out, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -20,8 +20,9 @@ _lib = None
 
 # dtype codes, include/xgen_amd.h
 DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_E4M3, DTYPE_I8, DTYPE_I32, DTYPE_NONE = 0, 1, 2, 3, 4, 5, -1
-NORM_LAYER, NORM_RMS, NORM_SCALE_ONE_PLUS = 0, 1, 0x100
+NORM_LAYER, NORM_RMS, NORM_SCALE_ONE_PLUS, NORM_NONE = 0, 1, 0x100, -1
 ACT_NONE, ACT_GELU_TANH = 0, 1
+ROUTE_SOFTMAX, ROUTE_SIGMOID, ROUTE_MAX_EXPERTS, ROUTE_MAX_CHOICES = 0, 1, 512, 32
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 
 _TORCH_DTYPE = {
@@ -98,11 +99,26 @@ SIGNATURES = {
     "xgen_fp8_wire_decode_strided": (_c_int, [
         _c_int, _c_int, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr,
         _c_ptr]),
+    "xgen_residual_norm": (_c_int, [
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_int, _c_ptr, _c_int,
+        _c_float, _c_float, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_int, _c_ptr,
+        _c_ptr, _c_ptr]),
+    "xgen_route_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "xgen_route": (_c_int, [
+        _c_int, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr,
+        _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "xgen_grouped_matmul": (_c_int, [
+        _c_int, _c_int, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr,
+        _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_i64, _c_ptr]),
+    "xgen_expert_combine": (_c_int, [
+        _c_int, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64,
+        _c_ptr, _c_i64, _c_ptr, _c_ptr]),
 }
 
 
 # added within ABI version 1: a library from before them still loads
-ADDED = frozenset({"xgen_fp8_quantize_tensor"})
+ADDED = frozenset({"xgen_fp8_quantize_tensor", "xgen_residual_norm", "xgen_route", "xgen_route_workspace_bytes",
+                   "xgen_grouped_matmul", "xgen_expert_combine"})
 
 
 def library_path() -> Path:

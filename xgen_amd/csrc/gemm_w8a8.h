@@ -43,6 +43,16 @@ struct GemmArgs {
   uint32_t residual_bytes, gate_bytes;  // (M - 1) * ld_residual * 2 + N * 2, (gate_rows - 1) * gate_stride * 2 + N * 2
 };
 
+// A grouped call's arguments (grouped_gemm.hip): M is the rows of all groups, N, K and the strides are every
+// group's; a and its scales have a_rows rows.
+struct GroupedArgs : GemmArgs {
+  const int32_t *ends;  // [groups], on the device
+  const int32_t *rows;  // activation row of each output row, or null: the row itself
+  int groups;
+  int64_t a_rows;
+  int64_t w_group;      // bytes between two groups' weights
+};
+
 // Operand kinds of the kernel template.
 enum Kind { kInt8 = 0, kFp8 = 1, kFp8Exact = 2 };
 

@@ -12,8 +12,10 @@
 #include <dlfcn.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <cstdlib>
 #include <filesystem>
+#include <limits>
 #include <string>
 #include <tuple>
 
@@ -33,8 +35,11 @@ struct Api {
   X(xgen_gate_residual) X(xgen_indexed_modulate) X(xgen_merge_quant) X(xgen_w8a8_gate_residual)
 #define XGEN_FIELD(f) decltype(&::f) f;
   XGEN_API(XGEN_FIELD)
-  // added within ABI version 1: null where XGEN_AMD_LIBRARY names a library from before it
-  decltype(&::xgen_fp8_quantize_tensor) xgen_fp8_quantize_tensor;
+  // added within ABI version 1: null where XGEN_AMD_LIBRARY names a library from before them
+#define XGEN_ADDED(X)                                                                                       \
+  X(xgen_fp8_quantize_tensor) X(xgen_residual_norm) X(xgen_route_workspace_bytes) X(xgen_route)             \
+  X(xgen_grouped_matmul) X(xgen_expert_combine)
+  XGEN_ADDED(XGEN_FIELD)
 };
 
 Api open_api() {
@@ -58,8 +63,8 @@ Api open_api() {
   a.f = reinterpret_cast<decltype(&::f)>(dlsym(handle, #f));              \
   TORCH_CHECK(a.f, path, ": undefined symbol ", #f);
   XGEN_API(XGEN_RESOLVE)
-  a.xgen_fp8_quantize_tensor =
-      reinterpret_cast<decltype(&::xgen_fp8_quantize_tensor)>(dlsym(handle, "xgen_fp8_quantize_tensor"));
+#define XGEN_RESOLVE_ADDED(f) a.f = reinterpret_cast<decltype(&::f)>(dlsym(handle, #f));
+  XGEN_ADDED(XGEN_RESOLVE_ADDED)
   const auto version = reinterpret_cast<decltype(&::xgen_abi_version)>(dlsym(handle, "xgen_abi_version"));
   TORCH_CHECK(version && version() == XGEN_ABI_VERSION, path, ": unexpected ABI version");
   return a;
@@ -72,6 +77,13 @@ const Api &api() {
 
 void check(int status, const char *fn) {
   TORCH_CHECK(status == XGEN_OK, fn, ": ", api().xgen_status_string(status), ": ", api().xgen_last_error());
+}
+
+// An entry point of the ABI's additions that the opened library may lack.
+template <class Fn>
+Fn added(Fn fn, const char *name) {
+  TORCH_CHECK(fn, name, " is not in the xgen_amd library that XGEN_AMD_LIBRARY names: it is from before it; build a new one");
+  return fn;
 }
 
 int dtype_code(at::ScalarType t) {
@@ -408,6 +420,198 @@ std::tuple<Tensor, Tensor> merge_quant(const Tensor &x, at::ScalarType out_dtype
   return {q, scale};
 }
 
+// --- blocks with experts and sandwich norms ----------------------------------------------------
+// An optional vector or matrix as the kernels read it: contiguous, 16-byte aligned.
+Tensor optional_flat(const OptTensor &t) { return t ? aligned_flat(*t) : Tensor(); }
+const void *optional_ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+std::tuple<Tensor, Tensor, Tensor> residual_norm(const Tensor &residual_in, const Tensor &branch_in,
+                                                 const OptTensor &branch_weight, const OptTensor &weight,
+                                                 const OptTensor &gate_in, const OptTensor &scale_in,
+                                                 const OptTensor &shift_in, const OptTensor &indices_in,
+                                                 int64_t branch_norm, int64_t norm_kind, double residual_scale,
+                                                 double eps, at::ScalarType out_dtype) {
+  on_gpu(residual_in, branch_in, branch_weight, weight, gate_in, scale_in, shift_in, indices_in);
+  TORCH_CHECK(residual_in.dim() == 3 && branch_in.sizes() == residual_in.sizes() && residual_in.size(2) > 0 &&
+                  residual_in.scalar_type() == at::kBFloat16 && branch_in.scalar_type() == at::kBFloat16,
+              "residual_norm: BF16 residual/branch [B,S,H] required");
+  const int64_t B = residual_in.size(0), S = residual_in.size(1), H = residual_in.size(2);
+  TORCH_CHECK(H <= XGEN_NORM_MAX_WIDTH && H % 8 == 0, "residual_norm: H a multiple of 8, up to 8192, required");
+  for (const OptTensor *w : {&branch_weight, &weight})
+    TORCH_CHECK(!*w || ((*w)->dim() == 1 && (*w)->size(0) == H &&
+                        ((*w)->scalar_type() == at::kBFloat16 || (*w)->scalar_type() == at::kFloat)),
+                "residual_norm: BF16/F32 norm weights [H] or None required");
+  TORCH_CHECK(scale_in.has_value() == shift_in.has_value(), "residual_norm: scale and shift come together");
+  int64_t T = 0;
+  for (const OptTensor *t : {&gate_in, &scale_in, &shift_in}) {
+    if (!*t) continue;
+    TORCH_CHECK((*t)->dim() == 2 && (*t)->size(0) > 0 && (*t)->size(1) == H && (T == 0 || (*t)->size(0) == T) &&
+                    (*t)->scalar_type() == at::kBFloat16,
+                "residual_norm: BF16 tables [T,H] of one T required");
+    T = (*t)->size(0);
+  }
+  TORCH_CHECK(T == 0 || (indices_in && indices_in->dim() == 1 && indices_in->size(0) == S &&
+                         indices_in->scalar_type() == at::kLong),
+              "residual_norm: int64 indices [S] required with tables");
+  TORCH_CHECK(branch_norm == XGEN_NORM_NONE || branch_norm == XGEN_NORM_LAYER || branch_norm == XGEN_NORM_RMS,
+              "residual_norm: branch_norm must be -1 (none), 0 (layer) or 1 (rms)");
+  TORCH_CHECK(!branch_weight || branch_norm != XGEN_NORM_NONE, "residual_norm: a branch weight needs a branch norm");
+  TORCH_CHECK(norm_kind == XGEN_NORM_LAYER || norm_kind == XGEN_NORM_RMS,
+              "residual_norm: norm_kind must be 0 (layer) or 1 (rms)");
+  TORCH_CHECK(std::isfinite(residual_scale) && std::abs(residual_scale) <= std::numeric_limits<float>::max(),
+              "residual_norm: residual_scale must be finite");
+  TORCH_CHECK(0 < eps && eps < 1, "residual_norm: eps must be in (0, 1)");
+  TORCH_CHECK(out_dtype == at::kBFloat16 || is_quant(out_dtype),
+              "residual_norm: out_dtype must be bfloat16, float8_e4m3fn or int8");
+  const auto entry = added(api().xgen_residual_norm, "xgen_residual_norm");
+  const c10::DeviceGuard guard(residual_in.device());
+  const bool quantized = out_dtype != at::kBFloat16;
+  Tensor stream = empty({B, S, H}, at::kBFloat16, residual_in);
+  Tensor rows = quantized ? empty({B * S, H}, out_dtype, residual_in) : empty({B, S, H}, out_dtype, residual_in);
+  Tensor token_scale = empty({quantized ? B * S : 0}, at::kFloat, residual_in);
+  if (B * S == 0) return {stream, rows, token_scale};
+  const Tensor x = kernel_rows(residual_in, 8), y = kernel_rows(branch_in, 8);
+  Tensor wb = optional_flat(branch_weight), w = optional_flat(weight);
+  if (wb.defined() && w.defined() && wb.scalar_type() != w.scalar_type()) {  // one dtype for both: the wider, exactly
+    wb = wb.to(at::kFloat);
+    w = w.to(at::kFloat);
+  }
+  auto table = [](const OptTensor &t) { return t ? kernel_rows(*t, 8) : Tensor(); };
+  const Tensor gate = table(gate_in), scale = table(scale_in), shift = table(shift_in);
+  const Tensor indices = T ? indices_in->contiguous() : Tensor();
+  auto row_stride = [](const Tensor &t) { return t.defined() ? t.stride(0) : 0; };
+  check(entry(x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), y.stride(0), y.stride(1), B, S, H,
+              (int)branch_norm, optional_ptr(wb), (int)norm_kind, optional_ptr(w),
+              wb.defined()  ? dtype_code(wb.scalar_type())
+              : w.defined() ? dtype_code(w.scalar_type())
+                            : XGEN_DTYPE_NONE,
+              (float)residual_scale, (float)eps, optional_ptr(gate), row_stride(gate), optional_ptr(scale),
+              row_stride(scale), optional_ptr(shift), row_stride(shift), T,
+              T ? indices.data_ptr<int64_t>() : nullptr, stream.data_ptr(), dtype_code(out_dtype), rows.data_ptr(),
+              quantized ? token_scale.data_ptr<float>() : nullptr, stream_of(residual_in)),
+        "xgen_residual_norm");
+  return {stream, rows, token_scale};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor &logits_in, int64_t k, const OptTensor &bias,
+                                                         int64_t scoring, bool renormalize, int64_t first_expert,
+                                                         int64_t local_experts) {
+  on_gpu(logits_in, bias);
+  TORCH_CHECK(logits_in.dim() == 2 && (is_half(logits_in) || logits_in.scalar_type() == at::kFloat) &&
+                  logits_in.size(1) > 0,
+              "route: BF16/F16/F32 logits [T,E] required");
+  const int64_t T = logits_in.size(0), E = logits_in.size(1);
+  TORCH_CHECK(E <= XGEN_ROUTE_MAX_EXPERTS, "route: up to ", XGEN_ROUTE_MAX_EXPERTS, " experts");
+  TORCH_CHECK(0 < k && k <= E && k <= XGEN_ROUTE_MAX_CHOICES, "route: k must be in 1..min(E, ", XGEN_ROUTE_MAX_CHOICES, ")");
+  TORCH_CHECK(!bias || (bias->dim() == 1 && bias->size(0) == E && bias->scalar_type() == at::kFloat),
+              "route: float32 bias [E] or None required");
+  TORCH_CHECK(scoring == XGEN_ROUTE_SOFTMAX || scoring == XGEN_ROUTE_SIGMOID,
+              "route: scoring must be 0 (softmax) or 1 (sigmoid)");
+  TORCH_CHECK(0 <= first_expert && 0 < local_experts && local_experts <= E && first_expert <= E - local_experts,
+              "route: [first_expert, first_expert + local_experts) must be experts");
+  TORCH_CHECK(T <= 0x7fffffffLL / k, "route: T*k must be below 2^31");
+  const auto entry = added(api().xgen_route, "xgen_route");
+  const c10::DeviceGuard guard(logits_in.device());
+  Tensor weights = empty({T, k}, at::kFloat, logits_in), chosen = empty({T, k}, at::kInt, logits_in);
+  Tensor ends = empty({local_experts}, at::kInt, logits_in), rows = empty({T * k}, at::kInt, logits_in);
+  Tensor slots = empty({T, k}, at::kInt, logits_in);
+  if (T == 0) return {weights, chosen, ends.zero_(), rows, slots};
+  Tensor logits = logits_in;
+  if (logits.stride(1) != 1 || logits.stride(0) < E) logits = logits.contiguous();
+  const Tensor b = bias ? bias->contiguous() : Tensor();
+  const size_t bytes = added(api().xgen_route_workspace_bytes, "xgen_route_workspace_bytes")(T, local_experts);
+  Tensor ws = bytes ? empty({(int64_t)bytes}, at::kByte, logits_in) : Tensor();
+  check(entry(dtype_code(logits.scalar_type()), logits.data_ptr(), logits.stride(0), T, E, k,
+              b.defined() ? b.data_ptr<float>() : nullptr, (int)scoring, renormalize ? 1 : 0, first_expert,
+              local_experts, weights.data_ptr<float>(), chosen.data_ptr<int>(), ends.data_ptr<int>(),
+              rows.data_ptr<int>(), slots.data_ptr<int>(), bytes ? ws.data_ptr() : nullptr, bytes,
+              stream_of(logits)),
+        "xgen_route");
+  return {weights, chosen, ends, rows, slots};
+}
+
+Tensor grouped_matmul(const Tensor &a_in, const Tensor &a_scale_in, const Tensor &w_in, const Tensor &w_scale_in,
+                      const Tensor &ends_in, const OptTensor &rows_in, const OptTensor &bias_in,
+                      at::ScalarType out_dtype, int64_t activation, bool exact) {
+  on_gpu(a_in, a_scale_in, w_in, w_scale_in, ends_in, rows_in, bias_in);
+  TORCH_CHECK(is_quant(a_in.scalar_type()) && w_in.scalar_type() == a_in.scalar_type(),
+              "grouped_matmul: operands must both be float8_e4m3fn or both int8");
+  TORCH_CHECK(a_in.dim() == 2 && w_in.dim() == 3 && a_in.size(1) == w_in.size(2) && w_in.size(0) > 0,
+              "grouped_matmul: a [R,K] and w [G,N,K] required");
+  const int64_t R = a_in.size(0), K = a_in.size(1), G = w_in.size(0), Nf = w_in.size(1);
+  TORCH_CHECK(G <= XGEN_ROUTE_MAX_EXPERTS, "grouped_matmul: up to ", XGEN_ROUTE_MAX_EXPERTS, " groups");
+  TORCH_CHECK(K > 0 && Nf > 0 && K % 16 == 0 && Nf % 16 == 0, "grouped_matmul: K and N must be multiples of 16");
+  TORCH_CHECK(a_scale_in.scalar_type() == at::kFloat && (a_scale_in.numel() == 1 || a_scale_in.numel() == R),
+              "grouped_matmul: float32 activation scale with 1 or R elements required");
+  TORCH_CHECK(w_scale_in.scalar_type() == at::kFloat &&
+                  (w_scale_in.sizes() == at::IntArrayRef{G, Nf} || w_scale_in.sizes() == at::IntArrayRef{G}),
+              "grouped_matmul: float32 weight scale [G] or [G,N] required");
+  TORCH_CHECK(ends_in.dim() == 1 && ends_in.size(0) == G && ends_in.scalar_type() == at::kInt,
+              "grouped_matmul: int32 ends [G] required");
+  TORCH_CHECK(!rows_in || (rows_in->dim() == 1 && rows_in->scalar_type() == at::kInt),
+              "grouped_matmul: int32 rows [M] or None required");
+  TORCH_CHECK(!bias_in || (bias_in->sizes() == at::IntArrayRef{G, Nf} &&
+                           (is_half(*bias_in) || bias_in->scalar_type() == at::kFloat)),
+              "grouped_matmul: bias [G,N] of BF16/F16/F32 required");
+  TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kHalf,
+              "grouped_matmul: out_dtype must be bfloat16 or float16");
+  TORCH_CHECK(activation == XGEN_ACT_NONE || activation == XGEN_ACT_GELU_TANH,
+              "grouped_matmul: activation must be 0 (none) or 1 (gelu_tanh)");
+  TORCH_CHECK(!exact || a_in.scalar_type() == at::kFloat8_e4m3fn,
+              "grouped_matmul: exact accumulation applies to FP8 operands");
+  const auto entry = added(api().xgen_grouped_matmul, "xgen_grouped_matmul");
+  const c10::DeviceGuard guard(a_in.device());
+  const int64_t M = rows_in ? rows_in->size(0) : R;
+  Tensor out = empty({M, Nf}, out_dtype, a_in);
+  if (M == 0) return out;
+  const Tensor a = kernel_rows(a_in, 16), w = kernel_rows(w_in, 16);
+  const Tensor a_scale = a_scale_in.contiguous(), w_scale = w_scale_in.contiguous(), ends = ends_in.contiguous();
+  const Tensor rows = rows_in ? rows_in->contiguous() : Tensor(), bias = bias_in ? bias_in->contiguous() : Tensor();
+  check(entry(dtype_code(a.scalar_type()), exact ? 1 : 0, a.data_ptr(), a.stride(0), R, w.data_ptr(), w.stride(1),
+              w.stride(0), M, Nf, K, G, ends.data_ptr<int>(), rows.defined() ? rows.data_ptr<int>() : nullptr,
+              a_scale.data_ptr<float>(), a_scale.numel() == R && R > 1 ? 1 : 0, w_scale.data_ptr<float>(),
+              w_scale.dim() == 2 ? 1 : 0, optional_ptr(bias),
+              bias.defined() ? dtype_code(bias.scalar_type()) : XGEN_DTYPE_NONE, (int)activation, out.data_ptr(),
+              dtype_code(out_dtype), out.stride(0), stream_of(a)),
+        "xgen_grouped_matmul");
+  return out;
+}
+
+Tensor expert_combine(const Tensor &y_in, const Tensor &weights_in, const Tensor &slots_in, const OptTensor &residual_in,
+                      const OptTensor &gate_in, const OptTensor &indices_in) {
+  on_gpu(y_in, weights_in, slots_in, residual_in, gate_in, indices_in);
+  TORCH_CHECK(y_in.dim() == 2 && is_half(y_in) && y_in.size(1) > 0 && y_in.size(1) % 8 == 0,
+              "expert_combine: BF16/F16 y [M,H] with H a multiple of 8 required");
+  TORCH_CHECK(weights_in.dim() == 2 && weights_in.size(1) > 0 && weights_in.scalar_type() == at::kFloat &&
+                  slots_in.sizes() == weights_in.sizes() && slots_in.scalar_type() == at::kInt,
+              "expert_combine: float32 weights and int32 slots [T,k] required");
+  const int64_t T = weights_in.size(0), k = weights_in.size(1), H = y_in.size(1);
+  TORCH_CHECK(!residual_in || (residual_in->sizes() == at::IntArrayRef{T, H} &&
+                               residual_in->scalar_type() == y_in.scalar_type()),
+              "expert_combine: residual [T,H] of y's dtype or None required");
+  TORCH_CHECK(!gate_in || (residual_in && gate_in->dim() == 2 && gate_in->size(0) > 0 && gate_in->size(1) == H &&
+                           gate_in->scalar_type() == y_in.scalar_type()),
+              "expert_combine: a gate table [G,H] of y's dtype needs a residual");
+  TORCH_CHECK(!gate_in || (indices_in && indices_in->dim() == 1 && indices_in->scalar_type() == at::kLong &&
+                           indices_in->size(0) > 0 && T % indices_in->size(0) == 0),
+              "expert_combine: int64 indices [S] with T % S == 0 required with a gate table");
+  const auto entry = added(api().xgen_expert_combine, "xgen_expert_combine");
+  const c10::DeviceGuard guard(y_in.device());
+  Tensor out = empty({T, H}, y_in.scalar_type(), y_in);
+  if (T == 0) return out;
+  const Tensor y = kernel_rows(y_in, 8), weights = weights_in.contiguous(), slots = slots_in.contiguous();
+  const Tensor residual = residual_in ? kernel_rows(*residual_in, 8) : Tensor();
+  const Tensor gate = gate_in ? kernel_rows(*gate_in, 8) : Tensor();
+  const Tensor indices = gate_in ? indices_in->contiguous() : Tensor();
+  check(entry(dtype_code(y.scalar_type()), y.data_ptr(), y.stride(0), y.size(0), weights.data_ptr<float>(),
+              slots.data_ptr<int>(), T, k, H, optional_ptr(residual), residual.defined() ? residual.stride(0) : 0,
+              optional_ptr(gate), gate.defined() ? gate.stride(0) : 0, gate.defined() ? gate.size(0) : 0,
+              gate.defined() ? indices.data_ptr<int64_t>() : nullptr, gate.defined() ? indices.size(0) : 0,
+              out.data_ptr(), stream_of(y)),
+        "xgen_expert_combine");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(xgen_amd, CUDA, m) {
@@ -422,4 +626,8 @@ TORCH_LIBRARY_IMPL(xgen_amd, CUDA, m) {
   m.impl("gate_residual", gate_residual);
   m.impl("indexed_modulate", indexed_modulate);
   m.impl("merge_quant", merge_quant);
+  m.impl("residual_norm", residual_norm);
+  m.impl("route", route);
+  m.impl("grouped_matmul", grouped_matmul);
+  m.impl("expert_combine", expert_combine);
 }

@@ -20,7 +20,8 @@ the attributes below (h3_npu_fusion.py:196-273), so they keep that contract:
 
 Features map onto this package's modules: "norm_quant" -> nq2, "swiglu" ->
 swiglu_quant, "gate_residual" -> gate_residual, "merge_quant" -> merge_quant,
-"phaa_layout" -> phaa_layout, all in libxgen_amd.so.  The reference's other
+"phaa_layout" -> phaa_layout, and, beyond the reference's, "residual_norm" ->
+residual_norm and "experts" -> experts, all in libxgen_amd.so.  The reference's other
 features (rope, laser preprocessing) are attention work outside the W8A8
 linear path and always fall back.
 """
@@ -207,6 +208,8 @@ class Kernels:
         "phaa_layout": ("phaa_layout", None),
         "laser_preprocess": None,
         "merge_quant": ("merge_quant", None),
+        "residual_norm": ("residual_norm", None),
+        "experts": ("experts", None),
     }
 
     def __init__(self, diagnostics):

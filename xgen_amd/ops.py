@@ -12,6 +12,7 @@ Contract violations raise RuntimeError before any launch.
 """
 from __future__ import annotations
 
+import math
 import threading
 
 import torch
@@ -44,6 +45,19 @@ SCHEMAS = {
     "scaled_mm_gate_residual": (
         "scaled_mm_gate_residual(Tensor a, Tensor w, Tensor a_scale, Tensor w_scale, Tensor? bias, "
         "Tensor residual, Tensor gate_table, Tensor indices) -> Tensor"),
+    "residual_norm": (
+        "residual_norm(Tensor residual, Tensor branch, Tensor? branch_weight, Tensor? weight, Tensor? gate_table, "
+        "Tensor? scale, Tensor? shift, Tensor? indices, int branch_norm, int norm_kind, float residual_scale, "
+        "float eps, ScalarType out_dtype) -> (Tensor, Tensor, Tensor)"),
+    "route": (
+        "route(Tensor logits, int k, Tensor? bias, int scoring, bool renormalize, int first_expert, "
+        "int local_experts) -> (Tensor, Tensor, Tensor, Tensor, Tensor)"),
+    "grouped_matmul": (
+        "grouped_matmul(Tensor a, Tensor a_scale, Tensor w, Tensor w_scale, Tensor ends, Tensor? rows, Tensor? bias, "
+        "ScalarType out_dtype, int activation, bool exact) -> Tensor"),
+    "expert_combine": (
+        "expert_combine(Tensor y, Tensor weights, Tensor slots, Tensor? residual, Tensor? gate_table, "
+        "Tensor? indices) -> Tensor"),
 }
 
 
@@ -221,6 +235,100 @@ def _mm_gate_meta(a, w, a_scale, w_scale, bias, residual, gate_table, indices):
     return torch.empty((a.shape[0], w.shape[0]), dtype=torch.bfloat16, device=a.device)
 
 
+def _residual_norm_meta(residual, branch, branch_weight, weight, gate_table, scale, shift, indices, branch_norm,
+                        norm_kind, residual_scale, eps, out_dtype):
+    what = "residual_norm"
+    _require(residual.dim() == 3 and branch.shape == residual.shape and residual.shape[2] > 0
+             and residual.dtype == branch.dtype == torch.bfloat16, f"{what}: BF16 residual/branch [B,S,H] required")
+    B, S, H = residual.shape
+    _require(H <= 8192 and H % 8 == 0, f"{what}: H a multiple of 8, up to 8192, required")
+    for w in (branch_weight, weight):
+        _require(w is None or (w.dim() == 1 and w.shape[0] == H and w.dtype in (torch.bfloat16, torch.float32)),
+                 f"{what}: BF16/F32 norm weights [H] or None required")
+    _require((scale is None) == (shift is None), f"{what}: scale and shift come together")
+    tables = [t for t in (gate_table, scale, shift) if t is not None]
+    for t in tables:
+        _require(t.dim() == 2 and t.shape[0] > 0 and t.shape[1] == H and t.shape[0] == tables[0].shape[0]
+                 and t.dtype == torch.bfloat16, f"{what}: BF16 tables [T,H] of one T required")
+    _require(not tables or (indices is not None and indices.dim() == 1 and indices.shape[0] == S
+                            and indices.dtype == torch.int64), f"{what}: int64 indices [S] required with tables")
+    _require(branch_norm in (N.NORM_NONE, N.NORM_LAYER, N.NORM_RMS),
+             f"{what}: branch_norm must be -1 (none), 0 (layer) or 1 (rms)")
+    _require(branch_weight is None or branch_norm != N.NORM_NONE, f"{what}: a branch weight needs a branch norm")
+    _require(norm_kind in (N.NORM_LAYER, N.NORM_RMS), f"{what}: norm_kind must be 0 (layer) or 1 (rms)")
+    _require(math.isfinite(residual_scale) and abs(residual_scale) <= torch.finfo(torch.float32).max,
+             f"{what}: residual_scale must be finite")
+    _require(0 < eps < 1, f"{what}: eps must be in (0, 1)")
+    _require(out_dtype in (torch.bfloat16, torch.float8_e4m3fn, torch.int8),
+             f"{what}: out_dtype must be bfloat16, float8_e4m3fn or int8")
+    quantized = out_dtype != torch.bfloat16
+    dev = residual.device
+    return (torch.empty((B, S, H), dtype=torch.bfloat16, device=dev),
+            torch.empty((B * S, H) if quantized else (B, S, H), dtype=out_dtype, device=dev),
+            torch.empty((B * S,) if quantized else (0,), dtype=torch.float32, device=dev))
+
+
+def _route_meta(logits, k, bias, scoring, renormalize, first_expert, local_experts):
+    what = "route"
+    _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float16, torch.float32)
+             and logits.shape[1] > 0, f"{what}: BF16/F16/F32 logits [T,E] required")
+    T, E = logits.shape
+    _require(E <= N.ROUTE_MAX_EXPERTS, f"{what}: up to {N.ROUTE_MAX_EXPERTS} experts")
+    _require(0 < k <= E and k <= N.ROUTE_MAX_CHOICES, f"{what}: k must be in 1..min(E, {N.ROUTE_MAX_CHOICES})")
+    _require(bias is None or (bias.dim() == 1 and bias.shape[0] == E and bias.dtype == torch.float32),
+             f"{what}: float32 bias [E] or None required")
+    _require(scoring in (N.ROUTE_SOFTMAX, N.ROUTE_SIGMOID), f"{what}: scoring must be 0 (softmax) or 1 (sigmoid)")
+    _require(0 <= first_expert and 0 < local_experts and first_expert + local_experts <= E,
+             f"{what}: [first_expert, first_expert + local_experts) must be experts")
+    _require(T * k < 2 ** 31, f"{what}: T*k must be below 2^31")
+
+    def out(shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device=logits.device)
+    return out((T, k), torch.float32), out((T, k)), out((local_experts,)), out((T * k,)), out((T, k))
+
+
+def _grouped_meta(a, a_scale, w, w_scale, ends, rows, bias, out_dtype, activation, exact):
+    what = "grouped_matmul"
+    _require(a.dtype in (torch.float8_e4m3fn, torch.int8) and w.dtype == a.dtype,
+             f"{what}: operands must both be float8_e4m3fn or both int8")
+    _require(a.dim() == 2 and w.dim() == 3 and a.shape[1] == w.shape[2] and w.shape[0] > 0,
+             f"{what}: a [R,K] and w [G,N,K] required")
+    (R, K), (G, Nf) = a.shape, w.shape[:2]
+    _require(G <= N.ROUTE_MAX_EXPERTS, f"{what}: up to {N.ROUTE_MAX_EXPERTS} groups")
+    _require(K > 0 and Nf > 0 and K % 16 == 0 and Nf % 16 == 0, f"{what}: K and N must be multiples of 16")
+    _require(a_scale.dtype == torch.float32 and a_scale.numel() in (1, R),
+             f"{what}: float32 activation scale with 1 or R elements required")
+    _require(w_scale.dtype == torch.float32 and (w_scale.shape == (G, Nf) or w_scale.shape == (G,)),
+             f"{what}: float32 weight scale [G] or [G,N] required")
+    _require(ends.dim() == 1 and ends.shape[0] == G and ends.dtype == torch.int32, f"{what}: int32 ends [G] required")
+    _require(rows is None or (rows.dim() == 1 and rows.dtype == torch.int32), f"{what}: int32 rows [M] or None required")
+    _require(bias is None or (bias.shape == (G, Nf) and bias.dtype in (torch.bfloat16, torch.float16, torch.float32)),
+             f"{what}: bias [G,N] of BF16/F16/F32 required")
+    _require(out_dtype in (torch.bfloat16, torch.float16), f"{what}: out_dtype must be bfloat16 or float16")
+    _require(activation in (N.ACT_NONE, N.ACT_GELU_TANH), f"{what}: activation must be 0 (none) or 1 (gelu_tanh)")
+    _require(not exact or a.dtype == torch.float8_e4m3fn, f"{what}: exact accumulation applies to FP8 operands")
+    return torch.empty((R if rows is None else rows.shape[0], Nf), dtype=out_dtype, device=a.device)
+
+
+def _combine_meta(y, weights, slots, residual, gate_table, indices):
+    what = "expert_combine"
+    _require(y.dim() == 2 and y.dtype in (torch.bfloat16, torch.float16) and y.shape[1] > 0 and y.shape[1] % 8 == 0,
+             f"{what}: BF16/F16 y [M,H] with H a multiple of 8 required")
+    _require(weights.dim() == 2 and weights.shape[1] > 0 and weights.dtype == torch.float32
+             and slots.shape == weights.shape and slots.dtype == torch.int32,
+             f"{what}: float32 weights and int32 slots [T,k] required")
+    T, H = weights.shape[0], y.shape[1]
+    _require(residual is None or (residual.shape == (T, H) and residual.dtype == y.dtype),
+             f"{what}: residual [T,H] of y's dtype or None required")
+    _require(gate_table is None or (residual is not None and gate_table.dim() == 2 and gate_table.shape[0] > 0
+                                    and gate_table.shape[1] == H and gate_table.dtype == y.dtype),
+             f"{what}: a gate table [G,H] of y's dtype needs a residual")
+    _require(gate_table is None or (indices is not None and indices.dim() == 1 and indices.dtype == torch.int64
+                                    and indices.shape[0] > 0 and T % indices.shape[0] == 0),
+             f"{what}: int64 indices [S] with T % S == 0 required with a gate table")
+    return torch.empty((T, H), dtype=y.dtype, device=y.device)
+
+
 # --------------------------------------------------------------------------- device
 def _on_gpu(*ts):
     dev = ts[0].device
@@ -276,6 +384,10 @@ _META = {
     "merge_quant": _merge_meta,
     "swiglu_quant": _swiglu_meta,
     "scaled_mm_gate_residual": _mm_gate_meta,
+    "residual_norm": _residual_norm_meta,
+    "route": _route_meta,
+    "grouped_matmul": _grouped_meta,
+    "expert_combine": _combine_meta,
 }
 
 
