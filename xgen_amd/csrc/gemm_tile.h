@@ -58,66 +58,9 @@ struct TileCfg {
   static_assert(kLdsBytes <= 160 * 1024, "LDS");
 };
 
-// The tile of a grouped call that workgroup `block` of a grid of 8 per_xcd takes, or false: none.  Group e
-// is rows [ends[e - 1], ends[e]), each end taken within [0, M] and an end before its begin as an
-// empty group; the rows behind the last end are one more group (group == groups).  Tiles are numbered group by
-// group, so the counts' prefix sums find the group: every wave computes them, a lane a few consecutive
-// groups, with no LDS or barrier in front of the first loads.
-template <int BM, int BN>
-__device__ __forceinline__ bool grouped_tile(const GroupedArgs &p, int block, int &group, int &row0, int &rows, int &n0) {
-  constexpr int kMaxPer = (XGEN_ROUTE_MAX_EXPERTS + 1 + 63) / 64;
-  const int lane = threadIdx.x & 63, per = (p.groups + 1 + 63) / 64;
-  auto end_of = [&](int e) {  // (M from the rows behind the last group on)
-    const int v = e < p.groups ? p.ends[e] : p.M;
-    return v < 0 ? 0 : v > p.M ? p.M : v;
-  };
-  int end[kMaxPer + 1], sum = 0;
-#pragma unroll
-  for (int i = 0; i <= kMaxPer; ++i) {
-    end[i] = 0;
-    if (i <= per && lane * per + i > 0) end[i] = end_of(lane * per + i - 1);
-  }
-#pragma unroll
-  for (int i = 0; i < kMaxPer; ++i)
-    if (i < per && end[i + 1] > end[i]) sum += (end[i + 1] - end[i] + BM - 1) / BM;
-  uint32_t incl = (uint32_t)sum;  // inclusive prefix sum over the lanes
-  incl += dpp_u32<0x111>(0, incl);  // row_shr 1, 2, 4, 8
-  incl += dpp_u32<0x112>(0, incl);
-  incl += dpp_u32<0x114>(0, incl);
-  incl += dpp_u32<0x118>(0, incl);
-  incl += dpp_u32<kDppRowBcast15, 0xa>(0, incl);
-  incl += dpp_u32<kDppRowBcast31, 0xc>(0, incl);
-  const int total = __builtin_amdgcn_readlane((int)incl, 63) * p.tiles_n;
-  // XCD x owns a contiguous range of the tiles (consecutive workgroup ids go to the 8 XCDs round-robin)
-  const int per_xcd = (total + 7) >> 3, t = (block & 7) * per_xcd + (block >> 3);
-  if ((block >> 3) >= per_xcd || t >= total) return false;
-  const int mt = t / p.tiles_n;  // the tile's row of tiles among all groups'
-  int at = (int)incl - sum, mine = -1, first = 0, begin = 0, count = 0;
-#pragma unroll
-  for (int i = 0; i < kMaxPer; ++i) {
-    if (i < per && end[i + 1] > end[i]) {
-      const int tiles = (end[i + 1] - end[i] + BM - 1) / BM;
-      if (mt >= at && mt < at + tiles) mine = lane * per + i, first = at, begin = end[i], count = end[i + 1] - end[i];
-      at += tiles;
-    }
-  }
-  const int owner = __builtin_ctzll(__ballot(mine >= 0));
-  group = __builtin_amdgcn_readlane(mine, owner);
-  first = __builtin_amdgcn_readlane(first, owner);
-  begin = __builtin_amdgcn_readlane(begin, owner);
-  count = __builtin_amdgcn_readlane(count, owner);
-  int m0;
-  tile_origin<BM, BN>(t - first * p.tiles_n, (count + BM - 1) / BM, p.tiles_n, p.group_m, m0, n0);
-  row0 = begin + m0;
-  rows = count - m0 < BM ? count - m0 : BM;
-  return true;
-}
-
-// ARGS: GemmArgs, or GroupedArgs for a product over ragged groups of rows.
-template <int KIND, int WM, int WN, int FM, int FN, int SLOTS, bool GATED, class ARGS = GemmArgs>
+template <int KIND, int WM, int WN, int FM, int FN, int SLOTS, bool GATED>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * WM * WN, 64 * WM * WN), amdgpu_waves_per_eu(1)))
-void gemm_tile_kernel(ARGS p) {
-  constexpr bool kGrouped = std::is_same<ARGS, GroupedArgs>::value;
+void gemm_tile_kernel(GemmArgs p) {
   typedef TileCfg<WM, WN, FM, FN, SLOTS> C;
   typedef Mfma<KIND> T;
   typedef typename T::frag_t frag_t;
@@ -134,16 +77,10 @@ void gemm_tile_kernel(ARGS p) {
 
   // --- this workgroup's tile: consecutive workgroup ids go to the 8 XCDs round-robin,
   // XCD x owns a contiguous range of tiles ---
+  const int t = (blockIdx.x & 7) * p.per_xcd + (blockIdx.x >> 3);
+  if (t >= p.tiles_m * p.tiles_n) return;
   int m0, n0;
-  [[maybe_unused]] int group = 0, row0 = 0, rows = 0;
-  if constexpr (kGrouped) {
-    if (!grouped_tile<C::kM, C::kN>(p, blockIdx.x, group, row0, rows, n0)) return;
-    m0 = 0;
-  } else {
-    const int t = (blockIdx.x & 7) * p.per_xcd + (blockIdx.x >> 3);
-    if (t >= p.tiles_m * p.tiles_n) return;
-    tile_origin<C::kM, C::kN>(t, p.tiles_m, p.tiles_n, p.group_m, m0, n0);
-  }
+  tile_origin<C::kM, C::kN>(t, p.tiles_m, p.tiles_n, p.group_m, m0, n0);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -152,55 +89,18 @@ void gemm_tile_kernel(ARGS p) {
   auto rsrc = [](const void *base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)bytes, kBufferFlags);
   };
-  // a grouped tile's operands: its group's weight, scales and bias; the rows from its first one on
-  // (32-bit offsets then hold whatever M and the groups' weights come to)
-  const uint8_t *a_base = p.a, *w_base = p.w;
-  uint8_t *out_base = static_cast<uint8_t *>(p.out);
-  uint32_t a_bytes = p.a_bytes, out_bytes = p.out_bytes;
-  const float *sw_base = p.sw;
-  const uint8_t *bias_base = static_cast<const uint8_t *>(p.bias);
-  int M = p.M;
-  if constexpr (kGrouped) {
-    M = rows;
-    out_base += (int64_t)row0 * p.ldo * 2;
-    out_bytes = (uint32_t)(((int64_t)(rows - 1) * p.ldo + p.N) * 2);
-    if (group == p.groups) {  // behind the last group: zeros
-      const __amdgpu_buffer_rsrc_t rz = rsrc(out_base, out_bytes);
-      constexpr int kZeroChunks = C::kN / 8;
-      for (int c = tid; c < C::kM * kZeroChunks; c += C::kThreads) {
-        const int r = c / kZeroChunks, col = n0 + c % kZeroChunks * 8;
-        __builtin_amdgcn_raw_buffer_store_b128(
-            u32x4{0, 0, 0, 0}, rz, r < rows && col < p.N ? (uint32_t)(r * p.ldo + col) * 2 : kOutOfRange, 0, 0);
-      }
-      return;
-    }
-    w_base += (int64_t)group * p.w_group;
-    sw_base += p.sw_stride ? (int64_t)group * p.N : group;
-    if (bias_base) bias_base += (int64_t)group * p.N * (p.bias_dtype == XGEN_DTYPE_F32 ? 4 : 2);
-    if (!p.rows) {
-      a_base += (int64_t)row0 * p.lda;
-      a_bytes = (uint32_t)((int64_t)(rows - 1) * p.lda + p.K);
-    }
-  }
-  const __amdgpu_buffer_rsrc_t ra = rsrc(a_base, a_bytes), rw = rsrc(w_base, p.w_bytes);
+  const __amdgpu_buffer_rsrc_t ra = rsrc(p.a, p.a_bytes), rw = rsrc(p.w, p.w_bytes);
 
   // --- the epilogue's scales and bias: thread t holds token m0 + t's and feature n0 + t's
   // from here to the epilogue, which shares them through LDS ---
   static_assert(C::kM <= C::kThreads && C::kN <= C::kThreads, "one token and one feature per thread");
-  const int pm = min(m0 + tid, M - 1), pn = min(n0 + tid, p.N - 1);
-  float sa_t;
-  if constexpr (kGrouped) {
-    const int64_t r = p.rows ? p.rows[row0 + pm] : row0 + pm;
-    sa_t = r >= 0 && r < p.a_rows ? p.sa[p.sa_stride ? r : 0] : __builtin_nanf("");  // no such row: NaN
-  } else {
-    sa_t = p.sa[p.sa_stride ? pm : 0];
-  }
-  const float sw_t = sw_base[p.sw_stride ? pn : 0];
+  const int pm = min(m0 + tid, p.M - 1), pn = min(n0 + tid, p.N - 1);
+  const float sa_t = p.sa[p.sa_stride ? pm : 0], sw_t = p.sw[p.sw_stride ? pn : 0];
   float bias_t = 0.0f;
-  if (bias_base) {  // uniform
-    if (p.bias_dtype == XGEN_DTYPE_F32) bias_t = reinterpret_cast<const float *>(bias_base)[pn];
-    else if (p.bias_dtype == XGEN_DTYPE_F16) bias_t = (float)reinterpret_cast<const _Float16 *>(bias_base)[pn];
-    else bias_t = Half2<XGEN_DTYPE_BF16>::lo(reinterpret_cast<const uint16_t *>(bias_base)[pn]);
+  if (p.bias) {  // uniform
+    if (p.bias_dtype == XGEN_DTYPE_F32) bias_t = static_cast<const float *>(p.bias)[pn];
+    else if (p.bias_dtype == XGEN_DTYPE_F16) bias_t = (float)static_cast<const _Float16 *>(p.bias)[pn];
+    else bias_t = Half2<XGEN_DTYPE_BF16>::lo(static_cast<const uint16_t *>(p.bias)[pn]);
   }
 
   // --- global -> LDS DMA: lane l fills row (l >> 3) of an 8-row load, physical chunk
@@ -210,34 +110,19 @@ void gemm_tile_kernel(ARGS p) {
   const int ch = ((lane & 7) ^ (((wave & 1) << 2) | (lane >> 4))) * 16;
   const uint32_t offa = (uint32_t)(m0 + wave * 8 + (lane >> 3)) * (uint32_t)p.lda + ch;
   const uint32_t offw = (uint32_t)(n0 + wave * 8 + (lane >> 3)) * (uint32_t)p.ldw + ch;
-  // a grouped tile's activation rows, one per load (gathered, or its own: those past the tile's last
-  // one, or outside the activation, read zeros)
-  [[maybe_unused]] uint32_t offg[kGrouped ? C::kLoadsA : 1];
-  if constexpr (kGrouped) {
-#pragma unroll
-    for (int q = 0; q < C::kLoadsA; ++q) {
-      const int r = wave * 8 + (lane >> 3) + q * C::kWaves * 8;
-      int64_t at = r;
-      if (p.rows) at = r < rows ? p.rows[row0 + r] : -1;
-      offg[q] = r < rows && at >= 0 && (!p.rows || at < p.a_rows) ? (uint32_t)at * (uint32_t)p.lda + ch : kOutOfRange;
-    }
-  }
   int dma_k = 0;             // K byte of the next pair to load
   uint32_t dma_slot = 0;     // its slot's LDS offset
-  uint32_t oa = 0, ow = 0;   // its offsets, or out of range (grouped: oa is the K byte)
+  uint32_t oa = 0, ow = 0;   // its offsets, or out of range
   // (kOutOfRange + rows * ld stays out of range: the host keeps (M + 512) * lda below 2^32)
   auto issue_begin = [&]() {
     const bool live = dma_k + ch < p.K;
-    oa = live ? (kGrouped ? 0 : offa) + dma_k : kOutOfRange;
+    oa = live ? offa + dma_k : kOutOfRange;
     ow = live ? offw + dma_k : kOutOfRange;
     asm volatile("" : "+v"(oa), "+v"(ow));
   };
   auto issue_load = [&](int q) {
     uint8_t *dst = smem + dma_slot + wave * 1024;
-    // (grouped: both terms below 2^31 or kOutOfRange; `or` keeps either's high bit, which a sum of two would drop)
-    if (q < C::kLoadsA && kGrouped)
-      dma_load16(ra, dst + q * C::kWaves * 1024, (offg[kGrouped ? q : 0] + (oa & ~kOutOfRange)) | (oa & kOutOfRange));
-    else if (q < C::kLoadsA) dma_load16(ra, dst + q * C::kWaves * 1024, oa + (uint32_t)(q * C::kWaves * 8 * p.lda));
+    if (q < C::kLoadsA) dma_load16(ra, dst + q * C::kWaves * 1024, oa + (uint32_t)(q * C::kWaves * 8 * p.lda));
     else {
       const int r = q - C::kLoadsA;
       dma_load16(rw, dst + C::kM * 128 + r * C::kWaves * 1024, ow + (uint32_t)(r * C::kWaves * 8 * p.ldw));
@@ -376,7 +261,7 @@ void gemm_tile_kernel(ARGS p) {
   auto piece = [&](int q, uint32_t &row, uint32_t &col) {  // piece q of this thread: 8 columns of a row
     const int c = q * C::kThreads + tid;
     row = (uint32_t)(m0 + c / kChunks), col = (uint32_t)(n0 + c % kChunks * 8);
-    return row < (uint32_t)M && col < (uint32_t)p.N;
+    return row < (uint32_t)p.M && col < (uint32_t)p.N;
   };
   // (the rest, past what the registers hold beside the fragments, behind the rounding)
   constexpr int kResAhead = kSteps <= 16 ? kSteps : 8;
@@ -435,9 +320,9 @@ void gemm_tile_kernel(ARGS p) {
           }
           *reinterpret_cast<u32x2 *>(smem + ml * C::kRowPitch + nl * 2) =
               u32x2{pack_out<kOut>(y[0], y[1]), pack_out<kOut>(y[2], y[3])};
-          if (!kGrouped && p.acc_out) {
+          if (p.acc_out) {
             const int m = m0 + ml, n = n0 + nl;
-            if (m < M && n < p.N) {
+            if (m < p.M && n < p.N) {
               typedef typename std::conditional<KIND == kInt8, i32x4, f32x4>::type acc4_t;
               *reinterpret_cast<acc4_t *>(static_cast<uint8_t *>(p.acc_out) + ((int64_t)m * p.N + n) * 4) = acc4_t{
                   acc[i][j][gq * 4 + 0], acc[i][j][gq * 4 + 1], acc[i][j][gq * 4 + 2], acc[i][j][gq * 4 + 3]};
@@ -462,7 +347,7 @@ void gemm_tile_kernel(ARGS p) {
 
   // rows of 16-byte pieces, consecutive lanes on consecutive pieces of a row; rows past M
   // and columns past N are dropped (N is a multiple of 16)
-  const __amdgpu_buffer_rsrc_t ro = rsrc(out_base, out_bytes);
+  const __amdgpu_buffer_rsrc_t ro = rsrc(p.out, p.out_bytes);
   constexpr int kUnroll = kSteps % 4 == 0 ? 4 : kSteps % 3 == 0 ? 3 : kSteps % 2 == 0 ? 2 : 1;
   [[maybe_unused]] u32x4 gt[GATED ? 2 : 1][kUnroll];  // the gate rows' pieces, one group ahead
   [[maybe_unused]] auto load_gate = [&](int q0) {
