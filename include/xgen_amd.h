@@ -494,11 +494,11 @@ int xgen_residual_norm(const void *x, int64_t x_stride_batch, int64_t x_stride_s
  * Pairs of the experts [first_expert, first_expert + local_experts) are ordered by (expert, token,
  * choice): ends int32 [local_experts] the pairs up to each one's last; rows int32 [tokens * k] the token
  * of each pair, -1 behind the last; slots int32 [tokens, k] the place of each pair, -1 without one.
- * The same on every run.  workspace: xgen_route_workspace_bytes(tokens, local_experts) bytes, 4-byte
+ * The same on every run.  workspace: xgen_route_workspace_bytes(tokens, experts, local_experts) bytes, 4-byte
  * aligned.  experts <= XGEN_ROUTE_MAX_EXPERTS, k <= min(experts, XGEN_ROUTE_MAX_CHOICES), tokens >= 1,
  * tokens * k < 2^31.
  */
-size_t xgen_route_workspace_bytes(int64_t tokens, int64_t local_experts);
+size_t xgen_route_workspace_bytes(int64_t tokens, int64_t experts, int64_t local_experts);
 int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t tokens, int64_t experts, int64_t k,
                const float *bias, int scoring, int renormalize, int64_t first_expert, int64_t local_experts,
                float *weights, int32_t *chosen, int32_t *ends, int32_t *rows, int32_t *slots, void *workspace,

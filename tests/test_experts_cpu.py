@@ -181,7 +181,7 @@ def call(fn, good, **changes):
 
 NORM = dict(x=16, xsb=0, xss=64, y=16, ysb=0, yss=64, batch=1, seq=4, width=64, bn=1, wb=16, kind=1, w=16, wdt=N.DTYPE_BF16, a=1.0, eps=1e-6,
             gate=16, gs=64, scale=16, ss=64, shift=16, ts=64, rows=3, idx=16, stream=16, out_dt=N.DTYPE_E4M3, out=16, tok=16, s=None)
-ROUTE = dict(dt=N.DTYPE_F32, x=16, ld=16, tokens=70, experts=16, k=2, bias=None, scoring=0, ren=1, first=0, local=16, w=16, c=16, e=16, r=16,
+ROUTE = dict(dt=N.DTYPE_F32, x=16, ld=16, tokens=300, experts=16, k=2, bias=None, scoring=0, ren=1, first=0, local=16, w=16, c=16, e=16, r=16,
              sl=16, ws=16, wsb=1 << 20, s=None)
 GROUPED = dict(dt=N.DTYPE_E4M3, exact=0, a=16, lda=32, ar=5, w=16, ldw=32, wg=1536, M=5, N=48, K=32, G=3, ends=16, rows=None, sa=16, sas=1, sw=16,
                sws=1, bias=None, bdt=N.DTYPE_NONE, act=0, out=16, odt=N.DTYPE_BF16, ldo=48, s=None)
@@ -236,5 +236,8 @@ def test_c_entries_without_work(built_library):
     assert call("xgen_residual_norm", NORM, seq=0, **nulls)(L) == N.OK
     assert call("xgen_grouped_matmul", GROUPED, M=0, ar=0, a=None, w=None, ends=None, sa=None, sw=None, out=None)(L) == N.OK
     assert call("xgen_expert_combine", COMBINE, tokens=0, y=None, w=None, sl=None, out=None, idx=None)(L) == N.OK
-    assert L.xgen_route_workspace_bytes(64, 16) == 0 and L.xgen_route_workspace_bytes(65, 16) == 2 * 16 * 4
-    assert L.xgen_route_workspace_bytes(32768, 8) == 512 * 32 and L.xgen_route_workspace_bytes(32769, 8) == 257 * 32
+    for experts, tokens in ((8, 32), (64, 32), (65, 16), (256, 8), (512, 4)):  # one launch up to there
+        assert L.xgen_route_workspace_bytes(tokens, experts, 16) == 0
+        assert L.xgen_route_workspace_bytes(tokens + 1, experts, 16) == -(-(tokens + 1) // 16) * 16 * 4
+    assert L.xgen_route_workspace_bytes(4096, 8, 8) == 256 * 32 and L.xgen_route_workspace_bytes(4097, 8, 8) == 65 * 32
+    assert L.xgen_route_workspace_bytes(32768, 8, 8) == 512 * 32 and L.xgen_route_workspace_bytes(32769, 8, 8) == 257 * 32

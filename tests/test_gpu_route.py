@@ -68,14 +68,15 @@ def logits(cuda, T, E, seed, dtype=torch.float32, scale=1.0):
                                  (200, 32), (256, 7), (257, 3), (512, 32)])
 def test_experts_and_choices(cuda, E, k, dtype):
     """bf16 logits repeat: ties go to the lowest expert."""
-    for T in (5, 131):
+    for T in (5, 131, 333):
         check(cuda, logits(cuda, T, E, E + k + T, dtype), k)
 
 
-@pytest.mark.parametrize("T", [1, 2, 63, 64, 65, 128, 129, 1000, 15624])
+@pytest.mark.parametrize("T", [1, 2, 8, 9, 16, 17, 32, 33, 63, 64, 65, 128, 129, 1000, 4096, 4097, 15624])
 def test_token_counts(cuda, T):
     check(cuda, logits(cuda, T, 64, T), 6, renormalize=False)
     check(cuda, logits(cuda, T, 8, T, torch.bfloat16), 2)
+    check(cuda, logits(cuda, T, 200, T), 5)
 
 
 def test_chunks_of_several_pieces(cuda):

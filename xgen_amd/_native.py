@@ -103,7 +103,7 @@ SIGNATURES = {
         _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_int, _c_ptr, _c_int,
         _c_float, _c_float, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_int, _c_ptr,
         _c_ptr, _c_ptr]),
-    "xgen_route_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
+    "xgen_route_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
     "xgen_route": (_c_int, [
         _c_int, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr,
         _c_ptr, _c_ptr, _c_ptr, _c_size, _c_ptr]),

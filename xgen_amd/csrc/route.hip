@@ -10,45 +10,79 @@
 //                rows[i]    token of pair i (-1 behind the last pair)
 //                slots[t,j] place of pair (t, j), or -1
 //
-// A chunk of tokens (64, more from 32,768 tokens on) is a workgroup's.  One chunk takes a single launch
-// that chooses, counts and places; more take two: every chunk's choices and its count per expert, then, from
-// all counts, every chunk's places.  Places are ranks (ballots within a wave, per-wave counts in LDS), never the order that an
-// atomic happened to take: the plan is the same on every run.
+// As many tokens as 4 waves choose for at once (32 of up to 64 experts, 4 of 512) take one launch that chooses, counts
+// and places; more take two: chunks of tokens choose and count their pairs per expert; then, from all counts, each
+// chunk places its own.  (16 tokens of 128 experts: 7.4 us, in two launches 5.2 + 4.2; 64 tokens: 11.3 us in one
+// launch of 16 waves, in two 5.8 + 4.4.)  Up to 4096 tokens a chunk is 16 tokens and a workgroup 4 waves, beyond 64
+// and 16: small workgroups spread the choosing over more CUs (4096 tokens 6.5 us against 10), but every one reads the
+// counts of all (7.2 us against 6).  Places are ranks (ballots within a wave, per-wave counts in LDS), never the order
+// that an atomic happened to take: the plan is the same on every run.
 //
-// A token is a group of G lanes with V logits each; a choice is a maximum over the group and a
-// ballot for the lowest expert that has it.
+// A token is a group of G lanes, a lane V consecutive experts.  A choice is the maximum over the group, the lowest
+// lane that has it and that lane's lowest expert with it, which it notes in LDS: nothing but the maximum crosses
+// lanes in the loop.  What bounds it is the issue of vector instructions (1 choice 8 us, 8 choices 12) and, below,
+// the launch and two dependent reads.  15,624 tokens, 128 experts, 8 choices, bf16: 10.5 us and the placement 6.8; a
+// wave per token, a ballot per logit and the counts read one by one took 14 and 12.
 #include "xgen_common.h"
 
 namespace xgen {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kChunk = 64;        // tokens that a workgroup takes at once
-constexpr int kMaxChunks = 512;   // every workgroup reads all chunks' counts: a chunk is several kChunk beyond
-constexpr int kMaxPairs = kChunk * XGEN_ROUTE_MAX_CHOICES;
+constexpr int kOneWaves = 4;      // one launch: waves of its workgroup
+constexpr int kPerWave = 4;       // two launches: tokens of a chunk per wave
+constexpr int kMaxChunks = 512;   // every workgroup reads all chunks' counts: a chunk is several passes beyond
 
 struct RouteArgs {
   const void *logits;
-  int dtype;
   int64_t ld;  // elements
   int64_t tokens;
   int experts, k;
   const float *bias;
   int sigmoid, renormalize;
+  int whole;  // logits can be read 8 at a time
   int first, local;
   float *weights;
   int32_t *chosen, *ends, *rows, *slots;
   int32_t *counts;  // [chunks][local]
   int chunks;
-  int64_t chunk_tokens;  // a multiple of kChunk
+  int64_t chunk_tokens;  // a multiple of kPerWave * waves
 };
 
-__device__ __forceinline__ float load_logit(const RouteArgs &a, int64_t t, int e) {
-  const int64_t i = t * a.ld + e;
-  if (a.dtype == XGEN_DTYPE_F32) return static_cast<const float *>(a.logits)[i];
-  const uint32_t w = static_cast<const uint16_t *>(a.logits)[i];
-  return a.dtype == XGEN_DTYPE_BF16 ? Half2<XGEN_DTYPE_BF16>::lo(w) : Half2<XGEN_DTYPE_F16>::lo(w);
+// V consecutive logits of a token's row from expert e0 on (those from `experts` on: -inf).  Whole: the row's pieces
+// are 16-byte aligned and no piece passes the experts.
+template <int DT, int V>
+__device__ __forceinline__ void load_logits(const RouteArgs &a, int64_t t, int e0, float (&x)[V]) {
+  using T = std::conditional_t<DT == XGEN_DTYPE_F32, float, uint16_t>;
+  const T *row = static_cast<const T *>(a.logits) + t * a.ld;
+  if constexpr (V == 8) {
+    if (a.whole) {  // uniform
+      // (the last piece's in place of those past it)
+      const T *piece = row + min(e0, a.experts - 8);
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(piece);
+      if constexpr (DT == XGEN_DTYPE_F32) {
+        const u32x4 u = *reinterpret_cast<const u32x4 *>(piece + 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[v] = __uint_as_float(w[v]), x[v + 4] = __uint_as_float(u[v]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[2 * v] = Half2<DT>::lo(w[v]), x[2 * v + 1] = Half2<DT>::hi(w[v]);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = e0 < a.experts ? x[v] : -__builtin_inff();
+      return;
+    }
+  }
+  // (the last expert's in place of those past it: loads under a condition each would wait for each other)
+  T w[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) w[v] = row[min(e0 + v, a.experts - 1)];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if constexpr (DT == XGEN_DTYPE_F32) x[v] = w[v];
+    else x[v] = Half2<DT>::lo((uint32_t)w[v]);
+    if (e0 + v >= a.experts) x[v] = -__builtin_inff();
+  }
 }
 
 // Reductions over groups of G lanes (every lane active), the result in every lane: quad
@@ -89,96 +123,118 @@ __device__ __forceinline__ float from_order_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// The choices of tokens [t0, t0 + kChunk), counted per expert into hist[local]; ids also into `ids`
-// ([token in chunk][k]) if given.
-template <int G, int V>
-__device__ __forceinline__ void choose(const RouteArgs &a, int64_t t0, int32_t *hist, int32_t *ids) {
+// What a taken expert's logit adds to its token's sum (-inf: nothing).
+__device__ __forceinline__ float score(float x, float top, int sigmoid) {
+  if (sigmoid) return 1.0f / (1.0f + expf(-x));
+  return x > -__builtin_inff() ? expf(x - top) : 0.0f;
+}
+
+// The choices of tokens [t0, t0 + n): expert j of token i at choice[i * k + j] (LDS), weights and experts out; pairs
+// counted per expert into hist[local].  logits: V per thread in LDS, a token's in the order of its experts.
+template <int DT, int G, int V, int WAVES>
+__device__ __forceinline__ void choose(const RouteArgs &a, int64_t t0, int n, int32_t *choice, float *logits,
+                                       int32_t *hist) {
   const int gl = threadIdx.x % G, lane = threadIdx.x & 63;
-  constexpr int kGroups = kThreads / G;
+  constexpr int kGroups = 64 * WAVES / G;
+  const uint64_t group = (G < 64 ? (1ull << (G & 63)) - 1 : ~0ull) << (lane & ~(G - 1));
+  const uint64_t before = group & ((1ull << lane) - 1);  // lanes of the group in front of this one
   const float ninf = -__builtin_inff();
-  const int n = (int)(a.tokens - t0 < kChunk ? a.tokens - t0 : kChunk);
-  float bias[V];
+  float bias[V] = {};
+  if (a.bias) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) bias[v] = a.bias && v * G + gl < a.experts ? a.bias[v * G + gl] : 0.0f;
-  for (int i0 = 0; i0 < n; i0 += kGroups) {  // (every lane stays active: tokens past the end redo the last one)
+    for (int v = 0; v < V; ++v) bias[v] = a.bias[min(gl * V + v, a.experts - 1)] + 0.0f;  // (never -0)
+  }
+  for (int i0 = 0; i0 < n; i0 += kGroups) {  // (every lane stays active: groups past the end redo the last token, unseen)
     const int i = i0 + (int)threadIdx.x / G;
-    const int64_t t = t0 + (i < n ? i : n - 1);
+    const bool live = i < n;
+    if (!__any(live)) break;
+    const int64_t t = t0 + (live ? i : n - 1);
     float x[V];
     uint32_t key[V];
+    load_logits<DT, V>(a, t, gl * V, x);
+#pragma unroll
+    for (int v = 0; v < V; ++v) logits[threadIdx.x * V + v] = x[v];
     bool nan = false;
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = v * G + gl < a.experts ? load_logit(a, t, v * G + gl) : ninf;
-#pragma unroll
     for (int v = 0; v < V; ++v) {
-      float s = a.bias ? x[v] + bias[v] : x[v];
-      if (s == 0.0f) s = 0.0f;  // -0 ranks with 0
-      key[v] = v * G + gl < a.experts && s > ninf ? order_key(s) : 0u;
+      const float s = x[v] + bias[v];  // (never -0, so that 0 and -0 rank alike)
+      key[v] = s > ninf ? order_key(s) : 0u;  // (-inf, NaN, no expert: 0)
       nan |= !(x[v] == x[v]);
     }
-    int mine = -1;  // lane j of the group: the group's choice j
+    nan = (__ballot(nan) & group) != 0;  // a NaN logit makes its token's weights NaN
+    int32_t *ids = choice + i * a.k;
+    uint32_t own = key[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) own = max_u32(own, key[v]);
     for (int j = 0; j < a.k; ++j) {
-      uint32_t m = key[0];
+      const uint32_t m = group_max<G>(own);
+      const uint64_t has = __ballot(own == m);
+      if (own == m && (has & before) == 0) {
+        int e = 0;
+        bool open = true;
+        own = 0;
 #pragma unroll
-      for (int v = 1; v < V; ++v) m = max_u32(m, key[v]);
-      m = group_max<G>(m);
-      int e = -1;
-#pragma unroll
-      for (int v = V - 1; v >= 0; --v) {
-        uint64_t at = __ballot(key[v] == m) >> (lane & ~(G - 1));
-        if constexpr (G < 64) at &= (1ull << G) - 1;
-        if (at) e = v * G + __builtin_ctzll(at);
+        for (int v = 0; v < V; ++v) {
+          const bool hit = open && key[v] == m;
+          e = hit ? v : e;
+          key[v] = hit ? 0 : key[v];
+          open = open && !hit;
+          own = max_u32(own, key[v]);
+        }
+        if (live) ids[j] = m ? gl * V + e : -1;
       }
-      if (m == 0) e = -1;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (e == v * G + gl) key[v] = 0;
-      if (gl == j) mine = e;
     }
-    // weights: the chosen experts' logits again (cached), one per lane
-    const bool taken = gl < a.k && mine >= 0;
-    const float xe = taken ? load_logit(a, t, mine) : ninf;
-    float p, total = 1.0f;
-    if (a.sigmoid) {
-      p = taken ? 1.0f / (1.0f + expf(-xe)) : 0.0f;
-      if (a.renormalize) total = group_sum<G>(p);
+    // the group's notes in LDS are in front of its reads: one wave, in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    auto logit = [&](int j) {  // of choice j, -inf for none
+      const int e = live && j < a.k ? ids[j] : -1;
+      return e < 0 ? ninf : logits[(threadIdx.x - gl) * V + e];
+    };
+    float top = ninf, total = 0.0f;
+    if (!a.renormalize) {  // over all experts
+      if (!a.sigmoid) {
+        float high = x[0];
+#pragma unroll
+        for (int v = 1; v < V; ++v) high = __builtin_fmaxf(high, x[v]);
+        top = from_order_key(group_max<G>(order_key(high)));
+#pragma unroll
+        for (int v = 0; v < V; ++v) total += x[v] > ninf ? expf(x[v] - top) : 0.0f;
+        total = group_sum<G>(total);
+      }
     } else {
-      // the peak over what is summed: the sum is 1 at least
-      float peak = xe;
-      if (!a.renormalize) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) peak = __builtin_fmaxf(peak, x[v]);
+      // over the choices; the peak is one of them, so the sum is 1 at least
+      if (!a.sigmoid) {
+        for (int j = gl; j < a.k; j += G) top = __builtin_fmaxf(top, logit(j));
+        top = from_order_key(group_max<G>(order_key(top)));
       }
-      peak = from_order_key(group_max<G>(order_key(peak)));
-      p = taken ? expf(xe - peak) : 0.0f;
-      if (a.renormalize) {
-        total = group_sum<G>(p);
-      } else {
-        float part = 0.0f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) part += x[v] > ninf ? expf(x[v] - peak) : 0.0f;
-        total = group_sum<G>(part);
-      }
+      for (int j = gl; j < a.k; j += G) total += score(logit(j), top, a.sigmoid);
+      total = group_sum<G>(total);
     }
-    // a NaN logit makes its token's weights NaN
-    nan = (__ballot(nan) >> (lane & ~(G - 1)) & (G < 64 ? (1ull << (G & 63)) - 1 : ~0ull)) != 0;
-    float w = taken ? (total > 0.0f ? p / total : total) : 0.0f;
-    if (nan && taken) w = __builtin_nanf("");
-    if (gl < a.k && i < n) {
-      a.chosen[t * a.k + gl] = mine;
-      a.weights[t * a.k + gl] = w;
-      if (ids) ids[i * a.k + gl] = mine;
-      const int le = mine - a.first;
-      if (mine >= 0 && le >= 0 && le < a.local) atomicAdd(&hist[le], 1);
+    if (!live) continue;
+    for (int j = gl; j < a.k; j += G) {
+      const int e = ids[j];
+      float w = 0.0f;
+      if (e >= 0) {
+        w = score(logit(j), top, a.sigmoid);
+        if (a.renormalize || !a.sigmoid) w = total > 0.0f ? w / total : total;
+        if (nan) w = __builtin_nanf("");
+        const int le = e - a.first;
+        if (le >= 0 && le < a.local) atomicAdd(&hist[le], 1);
+      }
+      a.chosen[t * a.k + j] = e;
+      a.weights[t * a.k + j] = w;
     }
   }
 }
 
-// LDS of the placement.
-struct PlaceShared {
-  int32_t count[kWaves][XGEN_ROUTE_MAX_EXPERTS];  // pairs of the wave's segment per expert; then its first place
+// What the placement keeps in LDS.
+template <int WAVES, int TOKENS>
+struct RouteShared {
+  static constexpr int kWaves = WAVES, kThreads = 64 * WAVES;
+  int32_t ids[TOKENS * XGEN_ROUTE_MAX_CHOICES];
+  int32_t count[WAVES * XGEN_ROUTE_MAX_EXPERTS];  // [wave][local]: pairs of the wave's segment; then its first place
   int32_t base[XGEN_ROUTE_MAX_EXPERTS];           // the chunk's first place per expert
   int32_t total[XGEN_ROUTE_MAX_EXPERTS];
-  int32_t ids[kMaxPairs];
   int32_t routed;                                 // pairs of all experts here
 };
 
@@ -195,7 +251,8 @@ __device__ __forceinline__ uint64_t same_group(int group, int bits) {
 
 // From every expert's pairs (sh.total) and those of the chunks before this one (sh.base): the group ends, and
 // the chunk's first place per expert into sh.base.
-__device__ __forceinline__ void first_places(const RouteArgs &a, bool write_ends, PlaceShared &sh) {
+template <class Shared>
+__device__ __forceinline__ void first_places(const RouteArgs &a, bool write_ends, Shared &sh) {
   const int lane = threadIdx.x & 63;
   __syncthreads();
   if (threadIdx.x < 64) {
@@ -227,12 +284,14 @@ __device__ __forceinline__ void first_places(const RouteArgs &a, bool write_ends
   }
 }
 
-// The places of tokens [t0, t0 + kChunk), whose choices are in sh.ids; sh.base moves on past them.
-__device__ __forceinline__ void place(const RouteArgs &a, int64_t t0, PlaceShared &sh) {
+// The places of the n pairs from token t0 on, whose choices are in sh.ids; sh.base moves on past them.
+template <class Shared>
+__device__ __forceinline__ void place(const RouteArgs &a, int64_t t0, int n, Shared &sh) {
+  constexpr int kWaves = Shared::kWaves, kThreads = Shared::kThreads;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = (int)(a.tokens - t0 < kChunk ? a.tokens - t0 : kChunk) * a.k;
-  for (int i = tid; i < kWaves * XGEN_ROUTE_MAX_EXPERTS; i += kThreads) (&sh.count[0][0])[i] = 0;
+  for (int i = tid; i < kWaves * a.local; i += kThreads) sh.count[i] = 0;
   __syncthreads();
+  int32_t *count = sh.count + wave * a.local;
   // each wave a contiguous segment of the pairs, 64 at a time
   const int seg = ((n + kWaves - 1) / kWaves + 63) / 64 * 64, begin = wave * seg;
   const int bits = 32 - __builtin_clz(a.local);  // groups 0 .. local (local: no expert here)
@@ -243,15 +302,15 @@ __device__ __forceinline__ void place(const RouteArgs &a, int64_t t0, PlaceShare
   for (int i0 = begin; i0 < begin + seg && i0 < n; i0 += 64) {
     const int g = group_of(i0 + lane);
     const uint64_t same = same_group(g, bits);
-    if (g < a.local && lane == __builtin_ctzll(same)) atomicAdd(&sh.count[wave][g], __builtin_popcountll(same));
+    if (g < a.local && lane == __builtin_ctzll(same)) atomicAdd(&count[g], __builtin_popcountll(same));
   }
   __syncthreads();
   for (int e = tid; e < a.local; e += kThreads) {
     int32_t at = sh.base[e];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const int32_t c = sh.count[w][e];
-      sh.count[w][e] = at;
+      const int32_t c = sh.count[w * a.local + e];
+      sh.count[w * a.local + e] = at;
       at += c;
     }
     sh.base[e] = at;
@@ -262,7 +321,7 @@ __device__ __forceinline__ void place(const RouteArgs &a, int64_t t0, PlaceShare
     const uint64_t same = same_group(g, bits);
     const int leader = __builtin_ctzll(same);
     int32_t at = 0;
-    if (g < a.local && lane == leader) at = atomicAdd(&sh.count[wave][g], __builtin_popcountll(same));
+    if (g < a.local && lane == leader) at = atomicAdd(&count[g], __builtin_popcountll(same));
     at = __shfl(at, leader) + (int32_t)__builtin_popcountll(same & ((1ull << lane) - 1));
     if (i < n) {
       const bool routed = g < a.local;
@@ -275,48 +334,80 @@ __device__ __forceinline__ void place(const RouteArgs &a, int64_t t0, PlaceShare
     if (i >= sh.routed) a.rows[i] = -1;
 }
 
-template <int G, int V>
-__global__ __launch_bounds__(kThreads) void route_one_kernel(RouteArgs a) {
-  __shared__ PlaceShared sh;
-  for (int e = threadIdx.x; e < a.local; e += kThreads) sh.total[e] = sh.base[e] = 0;
+template <int DT, int G, int V>
+__global__ __launch_bounds__(64 * kOneWaves) void route_one_kernel(RouteArgs a) {
+  __shared__ RouteShared<kOneWaves, 64 * kOneWaves / G> sh;
+  __shared__ __align__(16) float logits[64 * kOneWaves * V];
+  for (int e = threadIdx.x; e < a.local; e += 64 * kOneWaves) sh.total[e] = sh.base[e] = 0;
   __syncthreads();
-  choose<G, V>(a, 0, sh.total, sh.ids);
+  choose<DT, G, V, kOneWaves>(a, 0, (int)a.tokens, sh.ids, logits, sh.total);
   first_places(a, true, sh);
-  __syncthreads();
-  place(a, 0, sh);
+  place(a, 0, (int)a.tokens * a.k, sh);
 }
 
-template <int G, int V>
-__global__ __launch_bounds__(kThreads) void route_choose_kernel(RouteArgs a) {
-  __shared__ int32_t hist[XGEN_ROUTE_MAX_EXPERTS];
-  for (int e = threadIdx.x; e < a.local; e += kThreads) hist[e] = 0;
+template <int DT, int G, int V, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void route_choose_kernel(RouteArgs a) {
+  constexpr int kThreads = 64 * WAVES, kChunk = kPerWave * WAVES;
+  __shared__ int32_t ids[kChunk * XGEN_ROUTE_MAX_CHOICES], total[XGEN_ROUTE_MAX_EXPERTS];
+  __shared__ __align__(16) float logits[kThreads * V];
+  for (int e = threadIdx.x; e < a.local; e += kThreads) total[e] = 0;
   __syncthreads();
   const int64_t begin = (int64_t)blockIdx.x * a.chunk_tokens;
   const int64_t end = begin + a.chunk_tokens < a.tokens ? begin + a.chunk_tokens : a.tokens;
-  for (int64_t t0 = begin; t0 < end; t0 += kChunk) choose<G, V>(a, t0, hist, nullptr);
+  // (a wave's tokens are its own in LDS: no barrier between passes)
+  for (int64_t t0 = begin; t0 < end; t0 += kChunk)
+    choose<DT, G, V, WAVES>(a, t0, (int)(end - t0 < kChunk ? end - t0 : kChunk), ids, logits, total);
   __syncthreads();
-  for (int e = threadIdx.x; e < a.local; e += kThreads) a.counts[(int64_t)blockIdx.x * a.local + e] = hist[e];
+  for (int e = threadIdx.x; e < a.local; e += kThreads) a.counts[(int64_t)blockIdx.x * a.local + e] = total[e];
 }
 
-__global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a) {
-  __shared__ PlaceShared sh;
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
+  constexpr int kThreads = 64 * WAVES, kChunk = kPerWave * WAVES;
+  __shared__ RouteShared<WAVES, kChunk> sh;
   const int tid = threadIdx.x;
   for (int e = tid; e < a.local; e += kThreads) sh.total[e] = sh.base[e] = 0;
   __syncthreads();
-  // counts of all chunks and of those before this one: the threads share out the chunks
-  int span = 1;
-  while (span < a.local) span <<= 1;
-  const int e = tid & (span - 1), part = tid / span, parts = kThreads / span;
-  if (e < a.local) {
-    int32_t all = 0, before = 0;
-    for (int c = part; c < a.chunks; c += parts) {
-      const int32_t v = a.counts[(int64_t)c * a.local + e];
-      all += v;
-      before += c < (int)blockIdx.x ? v : 0;
+  // counts of all chunks and of those before this one: the threads share out the experts, four each where they
+  // divide, and the chunks
+  auto sum = [&](auto WIDTH) {
+    constexpr int W = decltype(WIDTH)::value;
+    using Counts = std::conditional_t<W == 4, i32x4, int32_t>;
+    const int columns = a.local / W;
+    int span = 1;
+    while (span < columns && span < kThreads) span <<= 1;
+    const int part = tid / span, parts = kThreads / span;
+    for (int c0 = 0; c0 < columns; c0 += span) {
+      const int c = c0 + (tid & (span - 1));
+      int32_t all[W] = {}, before[W] = {};
+      if (c < columns) {
+        constexpr int kDeep = 8;  // reads in flight (a missing chunk: one that is there, uncounted)
+        for (int i0 = part; i0 < a.chunks; i0 += kDeep * parts) {
+          Counts v[kDeep];
+#pragma unroll
+          for (int d = 0; d < kDeep; ++d)
+            v[d] = *reinterpret_cast<const Counts *>(a.counts + (int64_t)min(i0 + d * parts, a.chunks - 1) * a.local + c * W);
+#pragma unroll
+          for (int d = 0; d < kDeep; ++d) {
+            const int i = i0 + d * parts;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+              const int32_t n = reinterpret_cast<const int32_t *>(&v[d])[w];
+              all[w] += i < a.chunks ? n : 0;
+              before[w] += i < (int)blockIdx.x ? n : 0;
+            }
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          if (all[w]) atomicAdd(&sh.total[c * W + w], all[w]);
+          if (before[w]) atomicAdd(&sh.base[c * W + w], before[w]);
+        }
+      }
     }
-    if (all) atomicAdd(&sh.total[e], all);
-    if (before) atomicAdd(&sh.base[e], before);
-  }
+  };
+  if (a.local % 4 == 0 && (reinterpret_cast<uintptr_t>(a.counts) & 15) == 0) sum(std::integral_constant<int, 4>());
+  else sum(std::integral_constant<int, 1>());
   first_places(a, blockIdx.x == 0, sh);
   const int64_t begin = (int64_t)blockIdx.x * a.chunk_tokens;
   const int64_t end = begin + a.chunk_tokens < a.tokens ? begin + a.chunk_tokens : a.tokens;
@@ -324,26 +415,43 @@ __global__ __launch_bounds__(kThreads) void route_place_kernel(RouteArgs a) {
     const int n = (int)(end - t0 < kChunk ? end - t0 : kChunk) * a.k;
     __syncthreads();  // the places before are done with sh.ids
     for (int i = tid; i < n; i += kThreads) sh.ids[i] = a.chosen[t0 * a.k + i];
-    __syncthreads();
-    place(a, t0, sh);
+    place(a, t0, n, sh);
   }
 }
 
-template <int G, int V>
-void launch(const RouteArgs &a, hipStream_t stream) {
-  if (a.chunks == 1) {
-    route_one_kernel<G, V><<<dim3(1), dim3(kThreads), 0, stream>>>(a);
-    return;
-  }
-  route_choose_kernel<G, V><<<dim3((unsigned)a.chunks), dim3(kThreads), 0, stream>>>(a);
-  route_place_kernel<<<dim3((unsigned)a.chunks), dim3(kThreads), 0, stream>>>(a);
-}
-
+// Lanes of a token: 8 experts each, 8 lanes at least.
+int lanes_of(int64_t experts) { return experts <= 64 ? 8 : experts <= 128 ? 16 : experts <= 256 ? 32 : 64; }
+bool one_launch(int64_t tokens, int64_t experts) { return tokens <= kOneWaves * 64 / lanes_of(experts); }
+int waves_of(int64_t tokens) { return tokens <= 4096 ? 4 : 16; }
 int64_t chunk_tokens_of(int64_t tokens) {
-  const int64_t pieces = (tokens + kChunk - 1) / kChunk;
-  return (pieces + kMaxChunks - 1) / kMaxChunks * kChunk;
+  const int64_t pass = kPerWave * waves_of(tokens), pieces = (tokens + pass - 1) / pass;
+  return (pieces + kMaxChunks - 1) / kMaxChunks * pass;
 }
 int64_t chunks_of(int64_t tokens) { return (tokens + chunk_tokens_of(tokens) - 1) / chunk_tokens_of(tokens); }
+
+template <int DT, int G, int V>
+void launch(const RouteArgs &a, hipStream_t stream) {
+  const dim3 grid((unsigned)a.chunks);
+  if (one_launch(a.tokens, a.experts)) {
+    route_one_kernel<DT, G, V><<<dim3(1), dim3(64 * kOneWaves), 0, stream>>>(a);
+  } else if (waves_of(a.tokens) == 4) {
+    route_choose_kernel<DT, G, V, 4><<<grid, dim3(256), 0, stream>>>(a);
+    route_place_kernel<4><<<grid, dim3(256), 0, stream>>>(a);
+  } else {
+    route_choose_kernel<DT, G, V, 16><<<grid, dim3(1024), 0, stream>>>(a);
+    route_place_kernel<16><<<grid, dim3(1024), 0, stream>>>(a);
+  }
+}
+template <int DT>
+void launch(const RouteArgs &a, hipStream_t stream) {
+  if (a.experts <= 8) launch<DT, 8, 1>(a, stream);
+  else if (a.experts <= 16) launch<DT, 8, 2>(a, stream);
+  else if (a.experts <= 32) launch<DT, 8, 4>(a, stream);
+  else if (a.experts <= 64) launch<DT, 8, 8>(a, stream);
+  else if (a.experts <= 128) launch<DT, 16, 8>(a, stream);
+  else if (a.experts <= 256) launch<DT, 32, 8>(a, stream);
+  else launch<DT, 64, 8>(a, stream);
+}
 
 }  // namespace
 
@@ -351,8 +459,8 @@ int64_t chunks_of(int64_t tokens) { return (tokens + chunk_tokens_of(tokens) - 1
 
 using namespace xgen;
 
-extern "C" size_t xgen_route_workspace_bytes(int64_t tokens, int64_t local_experts) {
-  if (tokens <= kChunk || local_experts <= 0) return 0;
+extern "C" size_t xgen_route_workspace_bytes(int64_t tokens, int64_t experts, int64_t local_experts) {
+  if (tokens <= 0 || local_experts <= 0 || one_launch(tokens, experts)) return 0;
   return (size_t)chunks_of(tokens) * (size_t)local_experts * 4;
 }
 
@@ -377,13 +485,12 @@ extern "C" int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t 
   if (!logits || !weights || !chosen || !ends || !rows || !slots)
     return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
   if (tokens > 0x7fffffffLL / k) return fail(XGEN_ERR_UNSUPPORTED, "%s: tokens * k must be below 2^31", fn);
-  const size_t need = xgen_route_workspace_bytes(tokens, local_experts);
+  const size_t need = xgen_route_workspace_bytes(tokens, experts, local_experts);
   if (need && (!workspace || workspace_bytes < need))
     return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes required", fn, need);
 
   RouteArgs a;
   a.logits = logits;
-  a.dtype = in_dtype;
   a.ld = ld;
   a.tokens = tokens;
   a.experts = (int)experts;
@@ -401,14 +508,9 @@ extern "C" int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t 
   a.counts = static_cast<int32_t *>(workspace);
   a.chunks = (int)chunks_of(tokens);
   a.chunk_tokens = chunk_tokens_of(tokens);
-  // the fewest lanes that hold the experts, and the choices (one per lane)
-  const int64_t lanes = experts > k ? experts : k;
-  if (lanes <= 8) launch<8, 1>(a, stream);
-  else if (lanes <= 16) launch<16, 1>(a, stream);
-  else if (lanes <= 32) launch<32, 1>(a, stream);
-  else if (lanes <= 64) launch<64, 1>(a, stream);
-  else if (lanes <= 128) launch<64, 2>(a, stream);
-  else if (lanes <= 256) launch<64, 4>(a, stream);
-  else launch<64, 8>(a, stream);
+  a.whole = aligned16(logits) && ld % 8 == 0 && experts % 8 == 0;
+  if (in_dtype == XGEN_DTYPE_F32) launch<XGEN_DTYPE_F32>(a, stream);
+  else if (in_dtype == XGEN_DTYPE_BF16) launch<XGEN_DTYPE_BF16>(a, stream);
+  else launch<XGEN_DTYPE_F16>(a, stream);
   return launch_status(fn);
 }

@@ -519,7 +519,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor &logits_in
   Tensor logits = logits_in;
   if (logits.stride(1) != 1 || logits.stride(0) < E) logits = logits.contiguous();
   const Tensor b = bias ? bias->contiguous() : Tensor();
-  const size_t bytes = added(api().xgen_route_workspace_bytes, "xgen_route_workspace_bytes")(T, local_experts);
+  const size_t bytes = added(api().xgen_route_workspace_bytes, "xgen_route_workspace_bytes")(T, E, local_experts);
   Tensor ws = bytes ? empty({(int64_t)bytes}, at::kByte, logits_in) : Tensor();
   check(entry(dtype_code(logits.scalar_type()), logits.data_ptr(), logits.stride(0), T, E, k,
               b.defined() ? b.data_ptr<float>() : nullptr, (int)scoring, renormalize ? 1 : 0, first_expert,
