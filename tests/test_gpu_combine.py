@@ -37,7 +37,7 @@ def inputs(cuda, T, k, H, seed, dtype=torch.bfloat16, E=16, padded=0):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,k,H", [(1, 1, 8), (1, 8, 2048), (3, 3, 520), (64, 2, 512), (65, 5, 504), (7, 16, 5376),
-                                   (2000, 4, 1032)])
+                                   (2000, 4, 1032), (9000, 6, 2048)])
 def test_sizes(cuda, T, k, H, dtype):
     y, w, slots, g = inputs(cuda, T, k, H, T + H, dtype)
     check(cuda, y, w, slots)

@@ -180,6 +180,12 @@ def test_many_rows_of_a_long_sequence(cuda):
     check(cuda, x, y, FP8, **kw)
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, FP8])
+def test_a_call_past_the_last_level_cache(cuda, out):
+    x, y, kw = inputs(cuda, 1, 8000, 5376, seed=9)
+    check(cuda, x, y, out, **kw)
+
+
 def test_rows_past_32_bit_offsets(cuda):
     """x of 4.3 GB: rows whose byte offsets pass 2^32."""
     H, S = 8192, 262160

@@ -51,6 +51,7 @@ struct GroupedArgs : GemmArgs {
   int groups;
   int64_t a_rows;
   int64_t w_group;      // bytes between two groups' weights
+  bool past;            // operands and output pass the last-level cache
 };
 
 // Operand kinds of the kernel template.

@@ -308,16 +308,17 @@ void grouped_gemm_kernel(GroupedArgs p) {
       if (p.rows && !row_ok(index_set(set)[ml])) sa[j] = __builtin_nanf("");  // no such row
     }
     // The rows of a step (row block j, fragments i0 ..) are read back behind its writes and stored behind the next
-    // step's values: a wave's LDS operations complete in order.  Non-temporal: the output streams past the
-    // caches that the weights are re-read from (2,049 tokens x 8 of 128 experts, 2,048 x 1,536: 110 us, 105 so)
+    // step's values: a wave's LDS operations complete in order.  Non-temporal where the call's bytes pass the
+    // last-level cache (2,049 tokens x 8 of 128 experts, 2,048 x 1,536: 110 us, 105 so)
     u32x4 back[kBack];
     auto store = [&](int i0, int j) XGEN_INLINE {
 #pragma unroll
       for (int q = 0; q < kBack; ++q) {
         const int c = q * 64 + el, r = c / kPieces, col = c % kPieces;
         const int m = (j * WM + wm) * 32 + r, n = g.n0 + (wn * FN + i0) * 32 + col * 8;
-        __builtin_amdgcn_raw_buffer_store_b128(
-            back[q], ro, m < g.rows && n < p.N ? ((uint32_t)m * (uint32_t)p.ldo + (uint32_t)n) * 2 : kOutOfRange, 0, kCachePolicyNT);
+        const uint32_t at = m < g.rows && n < p.N ? ((uint32_t)m * (uint32_t)p.ldo + (uint32_t)n) * 2 : kOutOfRange;
+        if (p.past) __builtin_amdgcn_raw_buffer_store_b128(back[q], ro, at, 0, kCachePolicyNT);  // uniform
+        else __builtin_amdgcn_raw_buffer_store_b128(back[q], ro, at, 0, 0);
       }
     };
     each<FN / XF>([&](auto G) XGEN_INLINE {

@@ -216,6 +216,8 @@ extern "C" int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64
   g.groups = (int)groups;
   g.a_rows = a_rows;
   g.w_group = w_group_stride;
+  // (at most: groups may be empty)
+  g.past = (M < groups ? M : groups) * N * K + M * (2 * N + K) > kLastLevelCacheBytes;
   const int kind = in_dtype == XGEN_DTYPE_I8 ? kInt8 : exact ? kFp8Exact : kFp8;
   const int tile = choose_tile(kind, M, N, K, groups);
   if (kind == kInt8) return launch_kind<kInt8>(tile, g, stream);

@@ -14,7 +14,11 @@
 //
 // Layout: rows up to 1,024 values take a wave each, wider ones a workgroup of four waves, whose
 // reductions meet in LDS with one barrier each.  Workgroups as are resident at once walk the
-// rows; both norm weights stay in registers over the walk.
+// rows; both norm weights stay in registers over the walk.  Memory bound: 15,624 x 5,376 with gate, scale and shift
+// tables, bf16 out: 129 us, 5.2 TB/s (the rate of a large copy); e4m3fn out 120 us.  That call reads and writes past
+// the caches (129 us; through them 136).  Smaller ones go through them: at 4,000 rows past them is faster alone
+// (31 against 38 us), but slower with a kernel behind that reads both outputs (62.5 against 60).  A call of a few
+// hundred rows is its chain of loads and reductions, 5 us (501 rows 8).
 #include "fastdiv.h"
 #include "xgen_common.h"
 
@@ -99,7 +103,12 @@ struct NormWeight {
   }
 };
 
-template <int OUT, int WT, int WPR, int CH>
+__device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
+  return u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+}
+
+// PAST: the call's reads and writes pass the last-level cache
+template <int OUT, int WT, int WPR, int CH, bool PAST>
 __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) {
   static_assert(WPR == 1 || WPR == 4, "a wave or a workgroup per row");
   constexpr int kRowsPerBlock = 4 / WPR;
@@ -113,6 +122,19 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
 #pragma unroll
   for (int j = 0; j < CH; ++j) ok[j] = first + j * 64 * WPR < chunks;
 
+  // (rows past the end redo the last one, writing what its owner writes: the barriers stay in step)
+  auto row_at = [&](int64_t base) {
+    const int64_t want = base + wave / WPR;
+    return (uint32_t)(want < a.rows ? want : a.rows - 1);
+  };
+  // a row's table index: a scalar load (constant address space), a row ahead of the table rows it selects
+  auto index_of = [&](uint32_t row) -> int64_t {
+    const uint32_t s = row - fast_div(row, a.seq) * a.seq.d;
+    return a.indices ? ((const __attribute__((address_space(4))) int64_t *)a.indices)[s] : 0;
+  };
+  const int64_t step = (int64_t)gridDim.x * kRowsPerBlock;
+  int64_t next_g = index_of(row_at((int64_t)blockIdx.x * kRowsPerBlock));
+
   NormWeight<WT> wb[CH], wn[CH];
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
@@ -121,10 +143,8 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
   }
 
   int parity = 0;
-  // (rows past the end redo the last one, writing what its owner writes: the barriers stay in step)
-  for (int64_t base = (int64_t)blockIdx.x * kRowsPerBlock; base < a.rows; base += (int64_t)gridDim.x * kRowsPerBlock) {
-    const int64_t want = base + wave / WPR;
-    const uint32_t row = (uint32_t)(want < a.rows ? want : a.rows - 1);
+  for (int64_t base = (int64_t)blockIdx.x * kRowsPerBlock; base < a.rows; base += step) {
+    const uint32_t row = row_at(base);
     const uint32_t b = fast_div(row, a.seq), s = row - b * a.seq.d;
     const u32x4 *xr = reinterpret_cast<const u32x4 *>(a.x + (int64_t)b * a.xsb + (int64_t)s * a.xss);
     const u32x4 *yr = reinterpret_cast<const u32x4 *>(a.y + (int64_t)b * a.ysb + (int64_t)s * a.yss);
@@ -132,14 +152,15 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       xc[j] = yc[j] = u32x4{0, 0, 0, 0};
-      if (ok[j]) {
-        yc[j] = yr[first + j * 64 * WPR];
-        xc[j] = xr[first + j * 64 * WPR];
-      }
+      if (ok[j]) yc[j] = stream_load<PAST>(yr + first + j * 64 * WPR);
     }
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      if (ok[j]) xc[j] = stream_load<PAST>(xr + first + j * 64 * WPR);
     // table rows: gate 1, scale 0, shift 0 without a table; an index outside the tables makes what they
     // reach NaN (nothing outside is read)
-    const int64_t g = a.indices ? a.indices[s] : 0;
+    const int64_t g = next_g;
+    next_g = index_of(row_at(base + step));
     const bool g_ok = g >= 0 && g < a.table_rows;
     auto table = [&](const uint8_t *tab, int64_t stride, uint32_t none, u32x4 (&c)[CH]) {
       const uint32_t fill = tab && !g_ok ? 0x7fc07fc0u : none;
@@ -202,9 +223,7 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
 #pragma unroll
     for (int j = 0; j < CH; ++j)
       if (ok[j])
-        reinterpret_cast<u32x4 *>(so)[first + j * 64 * WPR] =
-            u32x4{pack_bf16x2(v[j][0], v[j][1]), pack_bf16x2(v[j][2], v[j][3]), pack_bf16x2(v[j][4], v[j][5]),
-                  pack_bf16x2(v[j][6], v[j][7])};
+        stream_store<PAST>(reinterpret_cast<u32x4 *>(so) + first + j * 64 * WPR, pack8(v[j]));
     statistics(v, a.norm, 2, mean, rstd);
     float am = 0.0f;
 #pragma unroll
@@ -226,9 +245,7 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
 #pragma unroll
       for (int j = 0; j < CH; ++j)
         if (ok[j])
-          reinterpret_cast<u32x4 *>(o)[first + j * 64 * WPR] =
-              u32x4{pack_bf16x2(v[j][0], v[j][1]), pack_bf16x2(v[j][2], v[j][3]), pack_bf16x2(v[j][4], v[j][5]),
-                    pack_bf16x2(v[j][6], v[j][7])};
+          stream_store<PAST>(reinterpret_cast<u32x4 *>(o) + first + j * 64 * WPR, pack8(v[j]));
     } else {
       const float amax = __uint_as_float(row_max<WPR>(__float_as_uint(am) & 0x7fffffffu, wave, lane, red.v[4]));
       RowQuant p;
@@ -241,19 +258,27 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
       uint8_t *o = a.out + (int64_t)row * a.width;
 #pragma unroll
       for (int j = 0; j < CH; ++j)
-        if (ok[j]) reinterpret_cast<u32x2 *>(o)[first + j * 64 * WPR] = quant8<OUT>(v[j], p);
+        if (ok[j]) stream_store<PAST>(reinterpret_cast<u32x2 *>(o) + first + j * 64 * WPR, quant8<OUT>(v[j], p));
       if (lane == 0 && wave % WPR == 0) a.token_scale[row] = p.s;
     }
   }
 }
 
-template <int OUT, int WT, int WPR, int CH>
-void launch(const ResNormArgs &a, hipStream_t stream) {
+template <int OUT, int WT, int WPR, int CH, bool PAST>
+void launch_walk(const ResNormArgs &a, hipStream_t stream) {
   constexpr int kRowsPerBlock = 4 / WPR;
-  static const int per_cu = resident_blocks_per_cu(residual_norm_kernel<OUT, WT, WPR, CH>, kThreads);
+  static const int per_cu = resident_blocks_per_cu(residual_norm_kernel<OUT, WT, WPR, CH, PAST>, kThreads);
   const int64_t need = (a.rows + kRowsPerBlock - 1) / kRowsPerBlock;
   const int64_t cap = (int64_t)device_cu_count() * per_cu;
-  residual_norm_kernel<OUT, WT, WPR, CH><<<dim3((unsigned)(need < cap ? need : cap)), dim3(kThreads), 0, stream>>>(a);
+  residual_norm_kernel<OUT, WT, WPR, CH, PAST>
+      <<<dim3((unsigned)(need < cap ? need : cap)), dim3(kThreads), 0, stream>>>(a);
+}
+
+template <int OUT, int WT, int WPR, int CH>
+void launch(const ResNormArgs &a, hipStream_t stream) {
+  // x, y and the stream, and the rows
+  if (a.rows * a.width * (OUT == XGEN_DTYPE_BF16 ? 8 : 7) > kLastLevelCacheBytes) launch_walk<OUT, WT, WPR, CH, true>(a, stream);
+  else launch_walk<OUT, WT, WPR, CH, false>(a, stream);
 }
 
 template <int OUT, int WT>

@@ -324,6 +324,19 @@ __device__ __forceinline__ uint32_t e4m3_slow_byte(float x, float s) {
   return pack_e4m3x4(clamp448(v), 0.0f, 0.0f, 0.0f) & 0xffu;
 }
 
+// Accesses of a streaming call: PAST, past the caches (its footprint passes the last level), or through them.  (A
+// template argument: of two branches on a run-time value the compiler makes one ordinary access.)
+template <bool PAST, class V>
+__device__ __forceinline__ V stream_load(const V *p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool PAST, class V>
+__device__ __forceinline__ void stream_store(V *p, V v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
 // Quantizes 8 values (bf16/f16 values as fp32) into 8 bytes.  No clamp is
 // needed on the E4M3 fast path: |x| <= amax and s = RN(amax / 448) bound the
 // quotient by 448 (1 + 2^-22), below 464, and v_cvt_pk_fp8_f32 rounds such

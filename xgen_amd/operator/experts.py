@@ -26,6 +26,8 @@ from .. import _native as N
 from ..ops import xops
 from .h3_fp8 import _ACCUMULATIONS, _ACTIVATIONS, _device_weight
 
+# (the overloads themselves: half a microsecond less a call)
+_route, _grouped_matmul, _combine = xops.route.default, xops.grouped_matmul.default, xops.expert_combine.default
 _SCORINGS = {"softmax": N.ROUTE_SOFTMAX, "sigmoid": N.ROUTE_SIGMOID}
 _FORMATS = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
 
@@ -36,8 +38,9 @@ def library_path():
 
 
 def _inference_only(*tensors):
-    if any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("the expert operators are inference-only; detach parameters explicitly")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("the expert operators are inference-only; detach parameters explicitly")
 
 
 class Routing(NamedTuple):
@@ -58,7 +61,7 @@ def route(logits, k, *, bias=None, scoring="softmax", renormalize=True, first_ex
         raise ValueError(f"scoring must be one of {sorted(_SCORINGS)}")
     if local_experts is None:
         local_experts = logits.shape[-1] - first_expert
-    return Routing(*xops.route(logits, k, bias, _SCORINGS[scoring], renormalize, first_expert, local_experts))
+    return Routing(*_route(logits, k, bias, _SCORINGS[scoring], renormalize, first_expert, local_experts))
 
 
 def grouped_matmul(q, scale, weight, weight_scale, ends, *, rows=None, bias=None, out_dtype=torch.bfloat16, activation=None,
@@ -73,8 +76,8 @@ def grouped_matmul(q, scale, weight, weight_scale, ends, *, rows=None, bias=None
         raise ValueError(f"unsupported activation {activation!r}")
     if accumulation not in _ACCUMULATIONS:
         raise ValueError(f"accumulation must be one of {_ACCUMULATIONS}")
-    return xops.grouped_matmul(q, scale, weight, weight_scale, ends, rows, bias, out_dtype, _ACTIVATIONS[activation],
-                               accumulation == "exact" and q.dtype == torch.float8_e4m3fn)
+    return _grouped_matmul(q, scale, weight, weight_scale, ends, rows, bias, out_dtype, _ACTIVATIONS[activation],
+                           accumulation == "exact" and q.dtype == torch.float8_e4m3fn)
 
 
 def combine(y, weights, slots, *, residual=None, gate_table=None, indices=None):
@@ -83,12 +86,12 @@ def combine(y, weights, slots, *, residual=None, gate_table=None, indices=None):
     table).  Shaped as the residual, [T, H] without one.  A slot of -1 adds nothing."""
     _inference_only(y, weights, residual, gate_table)
     if residual is None or residual.dim() == 2:
-        return xops.expert_combine(y, weights, slots, residual, gate_table, indices)
+        return _combine(y, weights, slots, residual, gate_table, indices)
     if residual.dim() != 3:
         raise ValueError("combine: residual [T, H] or [B, S, H] required")
     if gate_table is not None and (indices is None or indices.shape != (residual.shape[1],)):
         raise ValueError("combine: int64 indices [S] required with a gate table")
-    out = xops.expert_combine(y, weights, slots, residual.reshape(-1, residual.shape[2]), gate_table, indices)
+    out = _combine(y, weights, slots, residual.reshape(-1, residual.shape[2]), gate_table, indices)
     return out.reshape(residual.shape)
 
 

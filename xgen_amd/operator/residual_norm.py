@@ -22,6 +22,7 @@ import torch
 from .. import _native as N
 from ..ops import xops
 
+_residual_norm = xops.residual_norm.default  # (the overload itself: half a microsecond less a call)
 _NORMS = {"rms": N.NORM_RMS, "layer": N.NORM_LAYER}
 
 
@@ -33,12 +34,13 @@ def library_path():
 def residual_norm(residual, branch, *, branch_weight=None, gate_table=None, residual_scale=1.0, weight=None, scale=None,
                   shift=None, indices=None, branch_norm="rms", norm="rms", eps=1e-6, out_dtype=torch.bfloat16):
     """residual, branch BF16 [B, S, H]; weights BF16/F32 [H]; tables BF16 [T, H]; indices int64 [S]."""
-    for t in (residual, branch, branch_weight, gate_table, weight, scale, shift):
-        if t is not None and t.requires_grad:
-            raise ValueError("residual_norm is inference-only; detach parameters explicitly")
+    if (residual.requires_grad or branch.requires_grad or (branch_weight is not None and branch_weight.requires_grad)
+            or (weight is not None and weight.requires_grad) or (gate_table is not None and gate_table.requires_grad)
+            or (scale is not None and scale.requires_grad) or (shift is not None and shift.requires_grad)):
+        raise ValueError("residual_norm is inference-only; detach parameters explicitly")
     if norm not in _NORMS or (branch_norm is not None and branch_norm not in _NORMS):
         raise ValueError(f"norm must be one of {sorted(_NORMS)}, branch_norm one of them or None")
-    stream, rows, token_scale = xops.residual_norm(
+    stream, rows, token_scale = _residual_norm(
         residual, branch, branch_weight, weight, gate_table, scale, shift, indices,
         N.NORM_NONE if branch_norm is None else _NORMS[branch_norm], _NORMS[norm], float(residual_scale), float(eps),
         out_dtype)
