@@ -511,8 +511,8 @@ int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t tokens, int
  *   out[m, n] = out_dtype(acc * (a_scale[r] * w_scale[e, n]) + bias[e, n]),  acc = sum_k a[r, k] * w[e, n, k]
  * (with XGEN_ACT_GELU_TANH out_dtype(gelu_tanh(.)) of it) for row m of group e, r = rows[m], or m if rows is
  * NULL.  ends int32 [groups], on the device: group e is rows [ends[e - 1], ends[e]) (from 0); values are
- * taken within [0, M], a group whose end lies before its begin is empty.  Output rows behind the last
- * group's end are zeros.  a: [a_rows, K] of in_dtype (E4M3 or I8; exact: E4M3 products summed as
+ * taken within [0, M], and one below the one before as that one (the group is empty).  Output rows behind the
+ * last group's end are zeros.  a: [a_rows, K] of in_dtype (E4M3 or I8; exact: E4M3 products summed as
  * xgen_scaled_mm_fp8_exact); rows int32 [M] or NULL (a_rows = M); a row index outside [0, a_rows) gives a NaN
  * row.  w: [groups, N, K], rows ldw and groups w_group_stride elements apart.  a_scale_stride 0 or 1
  * (one scale, or a_rows); w_scale_stride 0 ([groups]) or 1 ([groups, N]).  bias: NULL or [groups, N].

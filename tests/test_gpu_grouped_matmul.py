@@ -141,6 +141,19 @@ def test_ends_are_taken_within_the_rows(cuda):
     assert torch.equal(grouped_matmul(**ref), grouped_matmul(**low))
 
 
+@pytest.mark.parametrize("G", [4, 200])
+def test_an_end_below_the_one_before_is_an_empty_group(cuda, G):
+    """No row has two groups, whatever the ends are: across a lane's groups and across lanes."""
+    given = [700 if e % 3 == 0 else 40 + e for e in range(G - 1)] + [710]
+    taken = [max(given[:e + 1]) for e in range(G)]
+    ops = operands(cuda, "int8", [0] * (G - 1) + [720], 720, 64, 64, seed=6)
+    got, ref = ({**ops, "ends": torch.tensor(ends, dtype=torch.int32, device=cuda)} for ends in (given, taken))
+    assert torch.equal(grouped_matmul(**got), grouped_matmul(**ref))
+    down = {**ops, "ends": torch.tensor([700] + [0] * (G - 1), dtype=torch.int32, device=cuda)}
+    flat = {**ops, "ends": torch.tensor([700] * G, dtype=torch.int32, device=cuda)}
+    assert torch.equal(grouped_matmul(**down), grouped_matmul(**flat))
+
+
 def test_nan_rows_stay_theirs(cuda):
     """NaN bytes (a poisoned token) reach their own rows only, in a group's last partial tile as well."""
     ops = operands(cuda, "fp8", [33, 40], 73, 64, 80, seed=6)

@@ -111,25 +111,35 @@ void grouped_gemm_kernel(GroupedArgs p) {
   int tile_rows, last_row;
   {
     constexpr int kMaxPer = XGEN_ROUTE_MAX_EXPERTS / 64;
-    // end[i + 1]: of group lane * per + i (past the last group: the last one's); end[0]: of the group before
+    // end[i + 1]: of group lane * per + i (past the last group: the last one's, or a lane's padding: the one before);
+    // end[0]: of the group before
     int end[kMaxPer + 1] = {}, sum = 0;
 #pragma unroll
     for (int i = 0; i < kMaxPer; ++i) {
       end[i + 1] = 0;
       if (i < per) end[i + 1] = p.ends[lane * per + i < p.groups ? lane * per + i : p.groups - 1];
     }
+    // within [0, M], and none below the one before: no row has two groups, and the tiles are as many as the host assumed
 #pragma unroll
     for (int i = 1; i <= kMaxPer; ++i) {
       end[i] = end[i] < 0 ? 0 : end[i] > p.M ? p.M : end[i];
-      if (i == per) end[0] = end[i];
+      end[i] = end[i] > end[i - 1] ? end[i] : end[i - 1];
     }
-    const int before = __shfl_up(end[0], 1);
-    end[0] = lane ? before : 0;
+    uint32_t top = (uint32_t)end[kMaxPer];  // inclusive prefix maximum over the lanes
+    top = max_u32(top, dpp_u32<0x111>(0, top));  // row_shr 1, 2, 4, 8
+    top = max_u32(top, dpp_u32<0x112>(0, top));
+    top = max_u32(top, dpp_u32<0x114>(0, top));
+    top = max_u32(top, dpp_u32<0x118>(0, top));
+    top = max_u32(top, dpp_u32<kDppRowBcast15, 0xa>(0, top));
+    top = max_u32(top, dpp_u32<kDppRowBcast31, 0xc>(0, top));
+    const int up = __shfl_up((int)top, 1), before = lane ? up : 0;
+#pragma unroll
+    for (int i = 0; i <= kMaxPer; ++i) end[i] = end[i] > before ? end[i] : before;
 #pragma unroll
     for (int i = 0; i < kMaxPer; ++i)
       if (i < per && end[i + 1] > end[i]) sum += (end[i + 1] - end[i] + C::kM - 1) / C::kM;
     uint32_t incl = (uint32_t)sum;  // inclusive prefix sum over the lanes
-    incl += dpp_u32<0x111>(0, incl);  // row_shr 1, 2, 4, 8
+    incl += dpp_u32<0x111>(0, incl);
     incl += dpp_u32<0x112>(0, incl);
     incl += dpp_u32<0x114>(0, incl);
     incl += dpp_u32<0x118>(0, incl);
