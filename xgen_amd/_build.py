@@ -62,7 +62,7 @@ def _operators() -> Path:
            "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{INCLUDE}", "-isystem", str(root / "include"), "-isystem", str(root / "include/torch/csrc/api/include"),
            "-isystem", str(rocm / "include"), str(CSRC / "torch_ops.cpp"), "-o", str(tmp),
-           f"-L{root / 'lib'}", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ldl"]
+           f"-L{root / 'lib'}", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_hip", "-ldl"]
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed for torch_ops.cpp:\n{proc.stdout}")

@@ -8,6 +8,7 @@
 // XGEN_AMD_LIBRARY or this library's own folder, as xgen_amd/_native.py opens it.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/library.h>
@@ -118,8 +119,9 @@ void on_gpu(const Tensor &first, const T &...rest) {
 
 hipStream_t stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
+// (at::empty's kernel itself, without its dispatch: 0.16 us less a tensor)
 Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor &like) {
-  return at::empty(sizes, like.options().dtype(dtype).memory_format(std::nullopt));
+  return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
 }
 
 // t [..., rows, cols] as the kernels read it: unit column stride, every outer stride a multiple of
