@@ -6,10 +6,17 @@ Tolerance of W8A8Experts against 64 bits: with e4m3 operands both of a product's
 their values (int8: half a unit of a row's largest / 127), so its relative 2-norm error is far below
 the sum of both for independent errors; 0.08 (int8 0.03) holds with room for two products and the
 activation.  The exact comparison is with the ungrouped operators."""
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
 import xgen_amd  # noqa: F401
+from conftest import library_without
+from xgen_amd import _native as N
 from xgen_amd.operator.experts import W8A8Experts, combine, route
 from xgen_amd.operator.residual_norm import residual_norm
 from xgen_amd.operator.runtime import Diagnostics, Kernels
@@ -219,3 +226,38 @@ def test_weights_on_the_cpu_stay_there(cuda):
     assert torch.equal(bits(on.up_weight), bits(other.up_weight)) and torch.equal(on.down_scale, other.down_scale)
     h, logits = torch.randn(5, 16, device=cuda).bfloat16(), torch.randn(5, 2, device=cuda)
     assert torch.equal(on(h, logits), other(h, logits))
+
+
+OLDER = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, xgen_amd
+from xgen_amd.operator.experts import combine, grouped_matmul, route
+from xgen_amd.operator.residual_norm import residual_norm
+x = torch.ones(1, 2, 16, dtype=torch.bfloat16, device="cuda")
+q, s = torch.ops.xgen_amd.quantize_rows(x[0], torch.int8)
+assert q.min().item() == 127
+plan = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+for call in (lambda: residual_norm(x, x), lambda: route(x[0].float(), 2),
+             lambda: grouped_matmul(q, s, q.reshape(1, 2, 16).repeat(1, 8, 1), s[:1], plan[:1, 0]),
+             lambda: combine(x[0], torch.ones(2, 1, device="cuda"), plan)):
+    try:
+        call()
+    except RuntimeError as error:
+        print(str(error).splitlines()[0])
+"""
+
+
+def test_library_from_before_the_operators(cuda, tmp_path):
+    """XGEN_AMD_LIBRARY names a library of this ABI version without the entry points: the other operators run on it, and
+    each of these names what it lacks."""
+    older = N.library_path()
+    symbols = ("xgen_residual_norm", "xgen_route", "xgen_grouped_matmul", "xgen_expert_combine")
+    for symbol in symbols:
+        folder = tmp_path / symbol
+        folder.mkdir()
+        older = library_without(older, symbol, folder)
+    proc = subprocess.run([sys.executable, "-c", OLDER, str(Path(__file__).resolve().parents[1])], check=True, timeout=100,
+                          stdout=subprocess.PIPE, text=True, env={**os.environ, "XGEN_AMD_LIBRARY": str(older)})
+    lines = proc.stdout.strip().splitlines()[-4:]
+    assert len(lines) == 4 and all(symbol in line for symbol, line in zip(symbols, lines)), lines
