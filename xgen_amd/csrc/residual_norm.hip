@@ -17,8 +17,8 @@
 // rows; both norm weights stay in registers over the walk.  Memory bound: 15,624 x 5,376 with gate, scale and shift
 // tables, bf16 out: 129 us, 5.2 TB/s (the rate of a large copy); e4m3fn out 120 us.  That call reads and writes past
 // the caches (129 us; through them 136).  Smaller ones go through them: at 4,000 rows past them is faster alone
-// (31 against 38 us), but slower with a kernel behind that reads both outputs (62.5 against 60).  A call of a few
-// hundred rows is its chain of loads and reductions, 5 us (501 rows 8).
+// (31 against 38 us), but slower with a kernel behind that reads both outputs (62.5 against 60).  One row takes
+// 4 us (the launch, its loads and reductions), and further rows what their bytes do: 256 rows 6, 501 rows 8.
 #include "fastdiv.h"
 #include "xgen_common.h"
 
@@ -79,19 +79,12 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, int wave, int lane, floa
 template <int WT>
 struct NormWeight {
   u32x4 w[WT == XGEN_DTYPE_F32 ? 2 : 1];
-  __device__ __forceinline__ void load(const void *base, int chunk, bool ok) {
-    if constexpr (WT == XGEN_DTYPE_F32) {
-      const uint32_t one = 0x3f800000u;
-      w[0] = w[1] = u32x4{one, one, one, one};
-      if (base && ok) {
-        w[0] = static_cast<const u32x4 *>(base)[2 * chunk];
-        w[1] = static_cast<const u32x4 *>(base)[2 * chunk + 1];
-      }
-    } else {
-      const uint32_t one = 0x3f803f80u;
-      w[0] = u32x4{one, one, one, one};
-      if (base && ok) w[0] = static_cast<const u32x4 *>(base)[chunk];
-    }
+  __device__ __forceinline__ void load(const void *base, int chunk) {
+    constexpr int kParts = WT == XGEN_DTYPE_F32 ? 2 : 1;
+    const uint32_t one = WT == XGEN_DTYPE_F32 ? 0x3f800000u : 0x3f803f80u;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
+      w[i] = base ? static_cast<const u32x4 *>(base)[kParts * chunk + i] : u32x4{one, one, one, one};
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     if constexpr (WT == XGEN_DTYPE_F32) {
@@ -118,9 +111,12 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
   const int first = (wave % WPR) * 64 + lane;  // this lane's first chunk of a row
   const float inv_w = 1.0f / (float)a.width;
   const int chunks = a.width >> 3;
-  bool ok[CH];
-#pragma unroll
-  for (int j = 0; j < CH; ++j) ok[j] = first + j * 64 * WPR < chunks;
+  // Every lane has its first CH - 1 chunks (a row's width is above what CH - 1 hold); the last may lie past the row's
+  // end: then the row's last chunk is read in its place, and counts nowhere.
+  const bool last = first + (CH - 1) * 64 * WPR < chunks;
+  const int last_at = last ? first + (CH - 1) * 64 * WPR : chunks - 1;
+  auto at = [&](int j) { return j < CH - 1 ? first + j * 64 * WPR : last_at; };
+  auto live = [&](int j) { return j < CH - 1 || last; };
 
   // (rows past the end redo the last one, writing what its owner writes: the barriers stay in step)
   auto row_at = [&](int64_t base) {
@@ -138,8 +134,8 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
   NormWeight<WT> wb[CH], wn[CH];
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
-    wb[j].load(a.branch_weight, first + j * 64 * WPR, ok[j]);
-    wn[j].load(a.weight, first + j * 64 * WPR, ok[j]);
+    wb[j].load(a.branch_weight, at(j));
+    wn[j].load(a.weight, at(j));
   }
 
   int parity = 0;
@@ -150,27 +146,23 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
     const u32x4 *yr = reinterpret_cast<const u32x4 *>(a.y + (int64_t)b * a.ysb + (int64_t)s * a.yss);
     u32x4 xc[CH], yc[CH], gc[CH], sc[CH], tc[CH];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      xc[j] = yc[j] = u32x4{0, 0, 0, 0};
-      if (ok[j]) yc[j] = stream_load<PAST>(yr + first + j * 64 * WPR);
-    }
+    for (int j = 0; j < CH; ++j) yc[j] = stream_load<PAST>(yr + at(j));
 #pragma unroll
-    for (int j = 0; j < CH; ++j)
-      if (ok[j]) xc[j] = stream_load<PAST>(xr + first + j * 64 * WPR);
+    for (int j = 0; j < CH; ++j) xc[j] = stream_load<PAST>(xr + at(j));
     // table rows: gate 1, scale 0, shift 0 without a table; an index outside the tables makes what they
     // reach NaN (nothing outside is read)
     const int64_t g = next_g;
     next_g = index_of(row_at(base + step));
     const bool g_ok = g >= 0 && g < a.table_rows;
     auto table = [&](const uint8_t *tab, int64_t stride, uint32_t none, u32x4 (&c)[CH]) {
-      const uint32_t fill = tab && !g_ok ? 0x7fc07fc0u : none;
-#pragma unroll
-      for (int j = 0; j < CH; ++j) c[j] = u32x4{fill, fill, fill, fill};
-      if (tab && g_ok) {
+      if (tab && g_ok) {  // uniform
         const u32x4 *r = reinterpret_cast<const u32x4 *>(tab + g * stride);
 #pragma unroll
-        for (int j = 0; j < CH; ++j)
-          if (ok[j]) c[j] = r[first + j * 64 * WPR];
+        for (int j = 0; j < CH; ++j) c[j] = r[at(j)];
+      } else {
+        const uint32_t fill = tab ? 0x7fc07fc0u : none;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) c[j] = u32x4{fill, fill, fill, fill};
       }
     };
     table(a.gate, a.gate_stride, 0x3f803f80u, gc);
@@ -179,29 +171,33 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
     Slots &red = slots[parity];
     parity ^= 1;
 
-    // statistics of v (zeros past the row's end): mean (layer norm) and 1 / sqrt(mean square + eps)
-    auto statistics = [&](const float (&v)[CH][8], int kind, int at, float &mean, float &rstd) {
+    // statistics of v: mean (layer norm) and 1 / sqrt(mean square + eps)
+    auto statistics = [&](const float (&v)[CH][8], int kind, int slot, float &mean, float &rstd) {
       mean = 0.0f;
+      float t[2] = {0.0f, 0.0f}, q[2] = {0.0f, 0.0f};
       if (kind == XGEN_NORM_LAYER) {
-        float t[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < CH; ++j)
+        for (int j = 0; j < CH; ++j) {
+          float u[2] = {t[0], t[1]};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) t[i & 1] += v[j][i];
-        mean = row_sum<WPR>(t[0] + t[1], wave, lane, red.v[at]) * inv_w;
+          for (int i = 0; i < 8; ++i) u[i & 1] += v[j][i];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) t[i] = live(j) ? u[i] : t[i];
+        }
+        mean = row_sum<WPR>(t[0] + t[1], wave, lane, red.v[slot]) * inv_w;
       }
-      float q[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
-        if (ok[j]) {
+        float u[2] = {q[0], q[1]};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float d = v[j][i] - mean;
-            q[i & 1] = __builtin_fmaf(d, d, q[i & 1]);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float d = v[j][i] - mean;
+          u[i & 1] = __builtin_fmaf(d, d, u[i & 1]);
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q[i] = live(j) ? u[i] : q[i];
       }
-      rstd = __builtin_amdgcn_rsqf(row_sum<WPR>(q[0] + q[1], wave, lane, red.v[at + 1]) * inv_w + a.eps);
+      rstd = __builtin_amdgcn_rsqf(row_sum<WPR>(q[0] + q[1], wave, lane, red.v[slot + 1]) * inv_w + a.eps);
     };
 
     float v[CH][8];
@@ -217,35 +213,33 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
       unpack8<XGEN_DTYPE_BF16>(gc[j], gv);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        v[j][i] = ok[j] ? __builtin_fmaf(a.residual_scale, xv[i], (v[j][i] - mean) * rstd * (wv[i] * gv[i])) : 0.0f;
+        v[j][i] = __builtin_fmaf(a.residual_scale, xv[i], (v[j][i] - mean) * rstd * (wv[i] * gv[i]));
     }
     uint8_t *so = a.stream + (int64_t)row * a.width * 2;
 #pragma unroll
     for (int j = 0; j < CH; ++j)
-      if (ok[j])
-        stream_store<PAST>(reinterpret_cast<u32x4 *>(so) + first + j * 64 * WPR, pack8(v[j]));
+      if (live(j)) stream_store<PAST>(reinterpret_cast<u32x4 *>(so) + at(j), pack8(v[j]));
     statistics(v, a.norm, 2, mean, rstd);
     float am = 0.0f;
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      if (ok[j]) {
-        float wv[8], sv[8], tv[8];
-        wn[j].get(wv);
-        unpack8<XGEN_DTYPE_BF16>(sc[j], sv);
-        unpack8<XGEN_DTYPE_BF16>(tc[j], tv);
+      float wv[8], sv[8], tv[8];
+      wn[j].get(wv);
+      unpack8<XGEN_DTYPE_BF16>(sc[j], sv);
+      unpack8<XGEN_DTYPE_BF16>(tc[j], tv);
+      float top = am;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[j][i] = __builtin_fmaf((v[j][i] - mean) * rstd * wv[i], 1.0f + sv[i], tv[i]);
-          am = __builtin_elementwise_maximum(am, __builtin_fabsf(v[j][i]));  // NaN-propagating
-        }
+      for (int i = 0; i < 8; ++i) {
+        v[j][i] = __builtin_fmaf((v[j][i] - mean) * rstd * wv[i], 1.0f + sv[i], tv[i]);
+        top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[j][i]));  // NaN-propagating
       }
+      am = live(j) ? top : am;
     }
     if constexpr (OUT == XGEN_DTYPE_BF16) {
       uint8_t *o = a.out + (int64_t)row * a.width * 2;
 #pragma unroll
       for (int j = 0; j < CH; ++j)
-        if (ok[j])
-          stream_store<PAST>(reinterpret_cast<u32x4 *>(o) + first + j * 64 * WPR, pack8(v[j]));
+        if (live(j)) stream_store<PAST>(reinterpret_cast<u32x4 *>(o) + at(j), pack8(v[j]));
     } else {
       const float amax = __uint_as_float(row_max<WPR>(__float_as_uint(am) & 0x7fffffffu, wave, lane, red.v[4]));
       RowQuant p;
@@ -258,7 +252,7 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(ResNormArgs a) 
       uint8_t *o = a.out + (int64_t)row * a.width;
 #pragma unroll
       for (int j = 0; j < CH; ++j)
-        if (ok[j]) stream_store<PAST>(reinterpret_cast<u32x2 *>(o) + first + j * 64 * WPR, quant8<OUT>(v[j], p));
+        if (live(j)) stream_store<PAST>(reinterpret_cast<u32x2 *>(o) + at(j), quant8<OUT>(v[j], p));
       if (lane == 0 && wave % WPR == 0) a.token_scale[row] = p.s;
     }
   }
