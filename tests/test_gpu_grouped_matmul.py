@@ -268,6 +268,20 @@ def test_every_tile(cuda, kind, case):
 
 
 @pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("most", [4, 24, 60, 110, 190])
+def test_weights_past_the_last_level_cache(cuda, kind, most):
+    """316 MB of weights, each read by about one tile row or by two: past the caches and through them."""
+    g = torch.Generator().manual_seed(most)
+    counts = torch.randint(1, most + 1, (96,), generator=g).tolist()
+    counts[5] = 0
+    M = sum(counts)
+    ops = operands(cuda, kind, counts, M, 2064, 1600, seed=most)
+    check(cuda, kind, ops)
+    rows = torch.randperm(M, generator=g).to(cuda, torch.int32)
+    check(cuda, kind, {**ops, "bias": None}, rows=rows, activation="gelu_tanh", out_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("kind", sorted(KINDS))
 def test_the_cases_above_take_every_tile(cuda, kind):
     taken = {tile_of(kind, sum(many_counts(c)), c[3], c[4], c[0]) for c in MANY}
     taken |= {tile_of(kind, c["M"], c["N"], c["K"], c["G"]) for c in (dict(M=9, N=2064, K=1040, G=3), dict(M=706, N=336, K=400, G=6))}

@@ -22,7 +22,7 @@
 // rows of all groups, numbered in order, are dealt out as the ungrouped kernel's tiles are: a contiguous
 // range per XCD, walked in groups of group_m tile rows of one expert.
 //
-// Few rows are bound by the weights (8 tokens x 6 of 64 experts, 2,816 x 2,048: 38 us, 5.3 TB/s), many by the matrix
+// Few rows are bound by the weights (8 tokens x 6 of 64 experts, 2,816 x 2,048: 35 us, 5.8 TB/s), many by the matrix
 // cores (31,248 rows of 8 experts, 14,336 x 5,376, FP8: 2.0 ms, 2.4 PFLOP/s, what one group of as many rows reaches).
 // Between them (2,049 tokens x 8 of 128 experts, 1,536 x 2,048: 105 us; without MFMAs and stores 89, without memory
 // 56) it is memory again: 504 MB read past the L2, 402 of them the weights, and 50 written, 5.3 TB/s.
@@ -38,6 +38,12 @@ namespace xgen {
 __device__ __forceinline__ void dma_load4(__amdgpu_buffer_rsrc_t rsrc, uint8_t *lds, uint32_t offset) {
   typedef __attribute__((address_space(3))) void *lds_ptr_t;
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)lds, 4, offset, 0, 0, 0);
+}
+
+// dma_load16 of what the call reads once: non-temporal.
+__device__ __forceinline__ void dma_load16_once(__amdgpu_buffer_rsrc_t rsrc, uint8_t *lds, uint32_t offset) {
+  typedef __attribute__((address_space(3))) void *lds_ptr_t;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)lds, 16, offset, 0, 0, kCachePolicyNT);
 }
 
 // f(0), f(1), .. f(N - 1) with the index a constant.
@@ -87,10 +93,11 @@ struct GroupTile {
   int group, row0, rows, n0;  // wave-uniform
 };
 
-// PLAIN: a bf16 output without activation; otherwise p.out_dtype and p.act say.
+// PLAIN: a bf16 output without activation; otherwise p.out_dtype and p.act say.  ONCE: the weights are read past the
+// caches (a branch on it at every load takes 1 us of 33).
 // (every lambda below is inlined: one that is not would hold what it captures in scratch memory)
 #define XGEN_INLINE __attribute__((always_inline))
-template <int KIND, int WM, int WN, int FM, int FN, int SLOTS, bool PLAIN>
+template <int KIND, int WM, int WN, int FM, int FN, int SLOTS, bool PLAIN, bool ONCE>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * WM * WN, 64 * WM * WN), amdgpu_waves_per_eu(1)))
 void grouped_gemm_kernel(GroupedArgs p) {
   typedef GroupedCfg<WM, WN, FM, FN, SLOTS> C;
@@ -267,8 +274,8 @@ void grouped_gemm_kernel(GroupedArgs p) {
       dma_load16(ra, dst + q * C::kWaves * 1024, live ? offa[q] + dma_k : kOutOfRange);
     } else {
       const int r = q - C::kLoadsA;
-      dma_load16(rw, dst + C::kM * 128 + r * C::kWaves * 1024,
-                 live ? offw + dma_k + (uint32_t)(r * C::kWaves * 8 * p.ldw) : kOutOfRange);
+      (ONCE ? dma_load16_once : dma_load16)(rw, dst + C::kM * 128 + r * C::kWaves * 1024,
+                                            live ? offw + dma_k + (uint32_t)(r * C::kWaves * 8 * p.ldw) : kOutOfRange);
     }
   };
   auto issue_end = [&]() XGEN_INLINE {
