@@ -209,7 +209,7 @@ extern "C" int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64
   g.N = (int)N;
   g.K = (int)K;
   g.sa = a_scale;
-  g.sa_stride = (int)a_scale_stride;
+  g.sa_stride = a_rows ? (int)a_scale_stride : 1;  // (of no rows there is no scale, not even a common one, to read)
   g.sw = w_scale;
   g.sw_stride = (int)w_scale_stride;
   g.bias = bias;
