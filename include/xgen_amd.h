@@ -516,7 +516,7 @@ int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t tokens, int
  * xgen_scaled_mm_fp8_exact); rows int32 [M] or NULL (a_rows = M); a row index outside [0, a_rows) gives a NaN
  * row.  w: [groups, N, K], rows ldw and groups w_group_stride elements apart.  a_scale_stride 0 or 1
  * (one scale, or a_rows); w_scale_stride 0 ([groups]) or 1 ([groups, N]).  bias: NULL or [groups, N].
- * out [M, N], rows ldo apart.  K, N multiples of 16, rows 16-byte aligned; one group's weight below
+ * out [M, N], rows ldo apart.  K, N multiples of 16, rows and the bias 16-byte aligned; one group's weight below
  * 2 GiB, and with rows the activation too; groups <= XGEN_ROUTE_MAX_EXPERTS.
  */
 int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64_t lda, int64_t a_rows, const void *w,

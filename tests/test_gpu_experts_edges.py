@@ -24,3 +24,24 @@ def test_rows_of_an_activation_without_rows(cuda, dtype, scales, M):
         out = grouped_matmul(q, torch.ones(scales, device=cuda), w, sw, ends, rows=rows)
         last = int(ends[-1])
         assert torch.isnan(out[:last].float()).all() and not out[last:].any()
+
+
+def aside(t, elements):
+    """t's values in a contiguous view `elements` into its storage."""
+    out = torch.empty(t.numel() + elements, dtype=t.dtype, device=t.device)[elements:].view(t.shape)
+    return out.copy_(t)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("elements", [1, 2, 3])
+def test_bias_at_an_odd_offset(cuda, dtype, elements):
+    """A contiguous bias whose base is not on 16 bytes (one of 16-bit values not on 4 either): the same bits."""
+    g = torch.Generator(device=cuda).manual_seed(elements)
+    q, w = torch.randint(-99, 99, (90, 64), generator=g, device=cuda), torch.randint(-99, 99, (3, 208, 64), generator=g, device=cuda)
+    s, ws = torch.rand((90,), generator=g, device=cuda), torch.rand((3, 208), generator=g, device=cuda) * 1e-3
+    ends = torch.tensor([7, 7, 90], dtype=torch.int32, device=cuda)
+    bias = torch.randn((3, 208), generator=g, device=cuda).to(dtype)
+    call = (q.to(torch.int8), s, w.to(torch.int8), ws, ends)
+    odd = aside(bias, elements)
+    assert odd.is_contiguous() and odd.data_ptr() % 16 and torch.equal(odd, bias)
+    assert torch.equal(grouped_matmul(*call, bias=odd), grouped_matmul(*call, bias=bias))

@@ -191,6 +191,7 @@ extern "C" int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64
   if (lda % 16 || ldw % 16 || w_group_stride % 16 || !aligned16(a) || !aligned16(w))
     return fail(XGEN_ERR_UNSUPPORTED, "%s: operand rows must be 16-byte aligned", fn);
   if (ldo % 8 || !aligned16(out)) return fail(XGEN_ERR_UNSUPPORTED, "%s: output rows must be 16-byte aligned", fn);
+  if (!aligned16(bias)) return fail(XGEN_ERR_UNSUPPORTED, "%s: the bias must be 16-byte aligned", fn);
   // 32-bit offsets: within one group's weight, one tile's rows and, gathered, the whole activation
   constexpr int64_t kLimit = 0x7fffffffLL;
   if (M > kLimit || N > kLimit / 2 || K > kLimit || ldw > 0xffffffffLL / (N + 512) || (N - 1) * ldw + K > kLimit)

@@ -568,7 +568,7 @@ Tensor grouped_matmul(const Tensor &a_in, const Tensor &a_scale_in, const Tensor
   if (M == 0) return out;
   const Tensor a = kernel_rows(a_in, 16), w = kernel_rows(w_in, 16);
   const Tensor a_scale = a_scale_in.contiguous(), w_scale = w_scale_in.contiguous(), ends = ends_in.contiguous();
-  const Tensor rows = rows_in ? rows_in->contiguous() : Tensor(), bias = bias_in ? bias_in->contiguous() : Tensor();
+  const Tensor rows = rows_in ? rows_in->contiguous() : Tensor(), bias = optional_flat(bias_in);
   check(entry(dtype_code(a.scalar_type()), exact ? 1 : 0, a.data_ptr(), a.stride(0), R, w.data_ptr(), w.stride(1),
               w.stride(0), M, Nf, K, G, ends.data_ptr<int>(), rows.defined() ? rows.data_ptr<int>() : nullptr,
               a_scale.data_ptr<float>(), a_scale.numel() == R && R > 1 ? 1 : 0, w_scale.data_ptr<float>(),
