@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import xgen_amd  # noqa: F401
-from xgen_amd.operator.experts import grouped_matmul
+from test_gpu_route import reference
+from xgen_amd.operator.experts import grouped_matmul, route
 
 pytestmark = pytest.mark.gpu
 FP8 = torch.float8_e4m3fn
@@ -45,3 +46,51 @@ def test_bias_at_an_odd_offset(cuda, dtype, elements):
     odd = aside(bias, elements)
     assert odd.is_contiguous() and odd.data_ptr() % 16 and torch.equal(odd, bias)
     assert torch.equal(grouped_matmul(*call, bias=odd), grouped_matmul(*call, bias=bias))
+
+
+# (the lowest and the highest logit of a token's row)
+LOW = [(-95.0, -90.0), (-104.0, -88.0), (-200.0, -150.0), (-3e4, -2.9e4), (-100.0, -60.0), (-80.0, -1.0), (-1.0, 0.5), (-120.0, 40.0)]
+
+
+def check_sigmoid(x, k, bias, renormalize):
+    """The plan is test_gpu_route's; the weights in 64 bits by the sigmoids' logarithms, which do not underflow.
+
+    Tolerance: as there (a sigmoid of a negative number is an exponential, a sum and a division, the sum below it one of k);
+    a subnormal result is rounded by half of 2^-149."""
+    got = route(x, k, bias=bias, scoring="sigmoid", renormalize=renormalize)
+    ref = reference(x, k, bias=bias, scoring="sigmoid", renormalize=renormalize)
+    for g, r in zip(got[1:], ref[1:]):
+        assert torch.equal(g.cpu().long(), r)
+    xd = x.double().cpu()
+    log = torch.nn.functional.logsigmoid(xd).gather(1, ref[1].clamp(min=0))
+    w = torch.softmax(log, 1) if renormalize else log.exp()
+    tol = (32 + xd.amax(1) - xd.amin(1))[:, None] * 2.0 ** -24
+    bad = (got.weights.cpu().double() - w).abs() > tol * w + 2.0 ** -149
+    assert not bad.any(), (xd[bad.any(1)], got.weights.cpu()[bad], w[bad])
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("E,k", [(4, 3), (60, 8), (300, 32)])
+@pytest.mark.parametrize("T", [len(LOW), 40 * len(LOW)])
+def test_sigmoid_scores_of_low_logits(cuda, T, E, k, dtype):
+    """Tokens whose sigmoids are subnormal or below every float: their quotients are not."""
+    g = torch.Generator(device=cuda).manual_seed(E + T)
+    lo, hi = torch.tensor(LOW * (T // len(LOW)), device=cuda).t()
+    x = (lo[:, None] + (hi - lo)[:, None] * torch.rand((T, E), generator=g, device=cuda)).to(dtype)
+    for bias in (None, torch.randn((E,), generator=g, device=cuda)):
+        got = check_sigmoid(x, k, bias, True)
+        assert ((got.weights.double().sum(1) - 1).abs() <= 40 * 2.0 ** -24).all()
+        check_sigmoid(x, k, bias, False)
+
+
+def test_sigmoid_scores_of_infinities(cuda):
+    """-inf takes no part, +inf scores 1, a token of -inf alone takes nothing."""
+    inf = float("inf")
+    x = torch.tensor([[-inf, -300.0, -inf, -301.0], [inf, -100.0, -inf, 0.0], [-inf] * 4], device=cuda)
+    for renormalize in (False, True):
+        got = route(x, 3, scoring="sigmoid", renormalize=renormalize)
+        assert got.experts.tolist() == [[1, 3, -1], [0, 3, 1], [-1] * 3] and not got.weights[2].any() and got.weights[0, 2] == 0
+        total = 1.5 if renormalize else 1.0
+        assert (got.weights[1, :2].double() - torch.tensor([1 / total, 0.5 / total], dtype=torch.float64, device=cuda)).abs().max() <= 2.0 ** -23
+    assert (got.weights[0, :2].double() - torch.sigmoid(torch.tensor([1.0, -1.0], dtype=torch.float64, device=cuda))).abs().max() <= 8 * 2.0 ** -24

@@ -123,10 +123,13 @@ __device__ __forceinline__ float from_order_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// What a taken expert's logit adds to its token's sum (-inf: nothing).
+// What an expert's logit adds to its token's sum (-inf: nothing), over a factor that is the same for all of a token:
+// softmax e^top; sigmoid 1 / (1 + e^-x) over e^min(top, 0), so that the sum of the taken ones is a half at least, however
+// low all of them are (1 / (1 + e^-x) itself is 0 from -88.8 on).  Without a sum, top is 0 and the factor 1.
 __device__ __forceinline__ float score(float x, float top, int sigmoid) {
-  if (sigmoid) return 1.0f / (1.0f + expf(-x));
-  return x > -__builtin_inff() ? expf(x - top) : 0.0f;
+  if (sigmoid && x >= 0.0f) return 1.0f / (1.0f + expf(-x));
+  const float e = x > -__builtin_inff() ? expf(x - (sigmoid ? __builtin_fminf(top, 0.0f) : top)) : 0.0f;
+  return sigmoid ? e / (1.0f + expf(x)) : e;
 }
 
 // The choices of tokens [t0, t0 + n): expert j of token i at choice[i * k + j] (LDS), weights and experts out; pairs
@@ -190,24 +193,21 @@ __device__ __forceinline__ void choose(const RouteArgs &a, int64_t t0, int n, in
       const int e = live && j < a.k ? ids[j] : -1;
       return e < 0 ? ninf : logits[(threadIdx.x - gl) * V + e];
     };
-    float top = ninf, total = 0.0f;
-    if (!a.renormalize) {  // over all experts
-      if (!a.sigmoid) {
-        float high = x[0];
-#pragma unroll
-        for (int v = 1; v < V; ++v) high = __builtin_fmaxf(high, x[v]);
-        top = from_order_key(group_max<G>(order_key(high)));
-#pragma unroll
-        for (int v = 0; v < V; ++v) total += x[v] > ninf ? expf(x[v] - top) : 0.0f;
-        total = group_sum<G>(total);
-      }
-    } else {
-      // over the choices; the peak is one of them, so the sum is 1 at least
-      if (!a.sigmoid) {
-        for (int j = gl; j < a.k; j += G) top = __builtin_fmaxf(top, logit(j));
-        top = from_order_key(group_max<G>(order_key(top)));
-      }
+    float top = a.sigmoid ? 0.0f : ninf, total = 0.0f;
+    if (a.renormalize) {
+      // over the choices; the peak is one of them
+      top = ninf;
+      for (int j = gl; j < a.k; j += G) top = __builtin_fmaxf(top, logit(j));
+      top = from_order_key(group_max<G>(order_key(top)));
       for (int j = gl; j < a.k; j += G) total += score(logit(j), top, a.sigmoid);
+      total = group_sum<G>(total);
+    } else if (!a.sigmoid) {  // over all experts
+      float high = x[0];
+#pragma unroll
+      for (int v = 1; v < V; ++v) high = __builtin_fmaxf(high, x[v]);
+      top = from_order_key(group_max<G>(order_key(high)));
+#pragma unroll
+      for (int v = 0; v < V; ++v) total += x[v] > ninf ? expf(x[v] - top) : 0.0f;
       total = group_sum<G>(total);
     }
     if (!live) continue;
