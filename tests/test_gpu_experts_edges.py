@@ -5,9 +5,10 @@ import torch
 
 import xgen_amd  # noqa: F401
 from test_gpu_route import reference
-from xgen_amd.operator.experts import grouped_matmul, route
+from xgen_amd.operator.experts import W8A8Experts, combine, grouped_matmul, route
 
 pytestmark = pytest.mark.gpu
+xops = torch.ops.xgen_amd
 FP8 = torch.float8_e4m3fn
 
 
@@ -94,3 +95,37 @@ def test_sigmoid_scores_of_infinities(cuda):
         total = 1.5 if renormalize else 1.0
         assert (got.weights[1, :2].double() - torch.tensor([1 / total, 0.5 / total], dtype=torch.float64, device=cuda)).abs().max() <= 2.0 ** -23
     assert (got.weights[0, :2].double() - torch.sigmoid(torch.tensor([1.0, -1.0], dtype=torch.float64, device=cuda))).abs().max() <= 8 * 2.0 ** -24
+
+
+def one_row(t):
+    """t [1, n] as a router's [n, 1] product transposed: strides (1, 1)."""
+    v = torch.empty((t.shape[1], 1), dtype=t.dtype, device=t.device).t().copy_(t)
+    assert v.shape == t.shape and v.stride() == (1, 1)
+    return v
+
+
+@pytest.mark.parametrize("E", [2, 24, 64, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_token_whose_row_stride_is_short(cuda, E, dtype):
+    """The stride between rows says nothing where there is one row."""
+    g = torch.Generator(device=cuda).manual_seed(E)
+    x = torch.randn((1, E), generator=g, device=cuda).to(dtype)
+    for a, b in zip(route(one_row(x), 2), route(x, 2)):
+        assert torch.equal(a, b)
+    wide = torch.randn((7, E), generator=g, device=cuda).to(dtype)
+    for a, b in zip(route(wide.as_strided((1, E), (0, 1)), 2), route(wide[:1], 2)):
+        assert torch.equal(a, b)
+
+
+def test_experts_of_one_token_whose_stride_is_short(cuda):
+    g = torch.Generator(device=cuda).manual_seed(2)
+    up, down = (torch.randn(s, generator=g, device=cuda).bfloat16() for s in ((4, 64, 48), (4, 48, 32)))
+    m = W8A8Experts(up, down, 2)
+    x, logits = torch.randn((1, 48), generator=g, device=cuda).bfloat16(), torch.randn((1, 4), generator=g, device=cuda)
+    ref = m(x, logits)
+    assert ref.any() and torch.equal(m(one_row(x), one_row(logits)), ref)
+    r = torch.randn((1, 48), generator=g, device=cuda).bfloat16()
+    assert torch.equal(m(x, logits, residual=one_row(r)), m(x, logits, residual=r))
+    y = torch.randn((1, 48), generator=g, device=cuda).bfloat16()
+    w, s = torch.ones((1, 1), device=cuda), torch.zeros((1, 1), dtype=torch.int32, device=cuda)
+    assert torch.equal(combine(one_row(y), w, s), y)

@@ -13,6 +13,7 @@
 #include <dlfcn.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <filesystem>
@@ -138,6 +139,10 @@ Tensor aligned_flat(const Tensor &t) {
   Tensor c = t.contiguous();
   return aligned16(c) ? c : c.clone();
 }
+
+// Elements between the rows of t [rows, cols], as an entry point takes them: at least a row's (a single row's stride
+// says nothing, and may be less).
+int64_t rows_apart(const Tensor &t) { return t.size(0) == 1 ? std::max(t.stride(0), t.size(1)) : t.stride(0); }
 
 // [..., K] -> [M, K] with unit last stride (copies only if needed).
 Tensor rows_view(const Tensor &x) {
@@ -519,11 +524,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor &logits_in
   Tensor slots = empty({T, k}, at::kInt, logits_in);
   if (T == 0) return {weights, chosen, ends.zero_(), rows, slots};
   Tensor logits = logits_in;
-  if (logits.stride(1) != 1 || logits.stride(0) < E) logits = logits.contiguous();
+  if (logits.stride(1) != 1 || (T > 1 && logits.stride(0) < E)) logits = logits.contiguous();
   const Tensor b = bias ? bias->contiguous() : Tensor();
   const size_t bytes = added(api().xgen_route_workspace_bytes, "xgen_route_workspace_bytes")(T, E, local_experts);
   Tensor ws = bytes ? empty({(int64_t)bytes}, at::kByte, logits_in) : Tensor();
-  check(entry(dtype_code(logits.scalar_type()), logits.data_ptr(), logits.stride(0), T, E, k,
+  check(entry(dtype_code(logits.scalar_type()), logits.data_ptr(), rows_apart(logits), T, E, k,
               b.defined() ? b.data_ptr<float>() : nullptr, (int)scoring, renormalize ? 1 : 0, first_expert,
               local_experts, weights.data_ptr<float>(), chosen.data_ptr<int>(), ends.data_ptr<int>(),
               rows.data_ptr<int>(), slots.data_ptr<int>(), bytes ? ws.data_ptr() : nullptr, bytes,
