@@ -117,6 +117,16 @@ def test_one_token_whose_row_stride_is_short(cuda, E, dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [torch.int8, FP8])
+@pytest.mark.parametrize("activation", [0, 1])
+def test_quantized_row_whose_stride_is_short(cuda, dtype, activation):
+    g = torch.Generator(device=cuda).manual_seed(1)
+    for H in (8, 50, 2048, 5376):
+        x = torch.randn((1, H), generator=g, device=cuda).bfloat16()
+        got, ref = xops.quantize_rows(one_row(x), dtype, activation), xops.quantize_rows(x, dtype, activation)
+        assert torch.equal(got[0].view(torch.uint8), ref[0].view(torch.uint8)) and torch.equal(got[1], ref[1])
+
+
 def test_experts_of_one_token_whose_stride_is_short(cuda):
     g = torch.Generator(device=cuda).manual_seed(2)
     up, down = (torch.randn(s, generator=g, device=cuda).bfloat16() for s in ((4, 64, 48), (4, 48, 32)))

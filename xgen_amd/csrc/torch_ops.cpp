@@ -165,7 +165,7 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor &x, at::ScalarType out_dty
   const Tensor m = rows_view(x);
   const bool gelu = activation == XGEN_ACT_GELU_TANH;
   check((gelu ? api().xgen_quantize_rows_gelu : api().xgen_quantize_rows)(
-            dtype_code(x.scalar_type()), m.data_ptr(), m.size(0), m.size(1), m.stride(0), dtype_code(out_dtype),
+            dtype_code(x.scalar_type()), m.data_ptr(), m.size(0), m.size(1), rows_apart(m), dtype_code(out_dtype),
             q.data_ptr(), m.size(1), scale.data_ptr<float>(), stream_of(x)),
         gelu ? "xgen_quantize_rows_gelu" : "xgen_quantize_rows");
   return {q, scale};
