@@ -471,7 +471,7 @@ int xgen_fp8_wire_decode_strided(int out_dtype, int streams, const void *wire, i
  * out (out_dtype BF16, E4M3 or I8): [batch, seq, width] contiguous; token_scale float32 [batch * seq]
  * (ignored for BF16).  An index outside the tables makes what its row takes from them NaN: the stream
  * if there is a gate, the rows in either case (quantized: NaN bytes or zeros, and a NaN scale).
- * width <= XGEN_NORM_MAX_WIDTH; width and strides multiples of 8, buffers 16-byte aligned.
+ * width <= XGEN_NORM_MAX_WIDTH; width and strides multiples of 8, buffers 16-byte aligned; eps in [2^-126, 1).
  */
 int xgen_residual_norm(const void *x, int64_t x_stride_batch, int64_t x_stride_seq, const void *branch,
                        int64_t br_stride_batch, int64_t br_stride_seq, int64_t batch, int64_t seq, int64_t width,

@@ -4,8 +4,11 @@ import pytest
 import torch
 
 import xgen_amd  # noqa: F401
+from test_experts_cpu import norm, outcome
+from test_experts_edges_cpu import EPS_REFUSED, EPS_TAKEN
 from test_gpu_route import reference
 from xgen_amd.operator.experts import W8A8Experts, combine, grouped_matmul, route
+from xgen_amd.operator.residual_norm import residual_norm
 
 pytestmark = pytest.mark.gpu
 xops = torch.ops.xgen_amd
@@ -139,3 +142,12 @@ def test_experts_of_one_token_whose_stride_is_short(cuda):
     y = torch.randn((1, 48), generator=g, device=cuda).bfloat16()
     w, s = torch.ones((1, 1), device=cuda), torch.zeros((1, 1), dtype=torch.int32, device=cuda)
     assert torch.equal(combine(one_row(y), w, s), y)
+
+
+@pytest.mark.parametrize("eps", EPS_TAKEN + EPS_REFUSED)
+def test_eps(cuda, eps):
+    assert outcome(norm(eps=eps), cuda) == outcome(norm(eps=eps), "meta")
+    z = torch.zeros((1, 3, 64), dtype=torch.bfloat16, device=cuda)
+    if eps in EPS_TAKEN:  # rows of zeros stay zeros
+        for kind in ("rms", "layer"):
+            assert not any(t.any() for t in residual_norm(z, z, norm=kind, branch_norm=kind, eps=eps))

@@ -324,7 +324,8 @@ extern "C" int xgen_residual_norm(const void *x, int64_t x_stride_batch, int64_t
   if (batch < 0 || seq < 0 || width <= 0 || (tables && table_rows <= 0))
     return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: bad shape batch=%lld seq=%lld width=%lld tables=%lld", fn,
                 (long long)batch, (long long)seq, (long long)width, (long long)table_rows);
-  if (!(eps > 0.0f && eps < 1.0f)) return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: eps must be in (0, 1)", fn);
+  // (v_rsq_f32 takes a subnormal for 0: a row of zeros would be 0 * inf)
+  if (!(eps >= kFltMin && eps < 1.0f)) return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: eps must be in [2^-126, 1)", fn);
   if (!__builtin_isfinite(residual_scale))
     return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: residual scale must be finite", fn);
   if (width > XGEN_NORM_MAX_WIDTH)

@@ -467,7 +467,8 @@ std::tuple<Tensor, Tensor, Tensor> residual_norm(const Tensor &residual_in, cons
               "residual_norm: norm_kind must be 0 (layer) or 1 (rms)");
   TORCH_CHECK(std::isfinite(residual_scale) && std::abs(residual_scale) <= std::numeric_limits<float>::max(),
               "residual_norm: residual_scale must be finite");
-  TORCH_CHECK(0 < eps && eps < 1, "residual_norm: eps must be in (0, 1)");
+  TORCH_CHECK((float)eps >= std::numeric_limits<float>::min() && (float)eps < 1.0f,
+              "residual_norm: eps must be in [2^-126, 1) as a float32");
   TORCH_CHECK(out_dtype == at::kBFloat16 || is_quant(out_dtype),
               "residual_norm: out_dtype must be bfloat16, float8_e4m3fn or int8");
   const auto entry = added(api().xgen_residual_norm, "xgen_residual_norm");

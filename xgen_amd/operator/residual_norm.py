@@ -33,7 +33,8 @@ def library_path():
 
 def residual_norm(residual, branch, *, branch_weight=None, gate_table=None, residual_scale=1.0, weight=None, scale=None,
                   shift=None, indices=None, branch_norm="rms", norm="rms", eps=1e-6, out_dtype=torch.bfloat16):
-    """residual, branch BF16 [B, S, H]; weights BF16/F32 [H]; tables BF16 [T, H]; indices int64 [S]."""
+    """residual, branch BF16 [B, S, H]; weights BF16/F32 [H]; tables BF16 [T, H]; indices int64 [S];
+    eps in [2^-126, 1)."""
     if (residual.requires_grad or branch.requires_grad or (branch_weight is not None and branch_weight.requires_grad)
             or (weight is not None and weight.requires_grad) or (gate_table is not None and gate_table.requires_grad)
             or (scale is not None and scale.requires_grad) or (shift is not None and shift.requires_grad)):

@@ -12,6 +12,7 @@ Contract violations raise RuntimeError before any launch.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 import threading
 
@@ -258,7 +259,8 @@ def _residual_norm_meta(residual, branch, branch_weight, weight, gate_table, sca
     _require(norm_kind in (N.NORM_LAYER, N.NORM_RMS), f"{what}: norm_kind must be 0 (layer) or 1 (rms)")
     _require(math.isfinite(residual_scale) and abs(residual_scale) <= torch.finfo(torch.float32).max,
              f"{what}: residual_scale must be finite")
-    _require(0 < eps < 1, f"{what}: eps must be in (0, 1)")
+    _require(torch.finfo(torch.float32).tiny <= ctypes.c_float(eps).value < 1,
+             f"{what}: eps must be in [2^-126, 1) as a float32")
     _require(out_dtype in (torch.bfloat16, torch.float8_e4m3fn, torch.int8),
              f"{what}: out_dtype must be bfloat16, float8_e4m3fn or int8")
     quantized = out_dtype != torch.bfloat16
