@@ -517,7 +517,7 @@ int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t tokens, int
  * row.  w: [groups, N, K], rows ldw and groups w_group_stride elements apart.  a_scale_stride 0 or 1
  * (one scale, or a_rows); w_scale_stride 0 ([groups]) or 1 ([groups, N]).  bias: NULL or [groups, N].
  * out [M, N], rows ldo apart.  K, N multiples of 16, rows and the bias 16-byte aligned; one group's weight below
- * 2 GiB, and with rows the activation too; groups <= XGEN_ROUTE_MAX_EXPERTS.
+ * 2 GiB, and with rows the activation too; M < 2^31 - 256; groups <= XGEN_ROUTE_MAX_EXPERTS.
  */
 int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64_t lda, int64_t a_rows, const void *w,
                         int64_t ldw, int64_t w_group_stride, int64_t M, int64_t N, int64_t K, int64_t groups,

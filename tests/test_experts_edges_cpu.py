@@ -33,3 +33,9 @@ def test_eps_taken(eps):
 def test_eps_refused(built_library, eps):
     assert outcome(norm(eps=eps), "meta") == ("refused", "residual_norm: eps must be in [2^-126, 1) as a float32")
     refused("xgen_residual_norm", NORM, dict(eps=eps), BAD, b"eps")
+
+
+@pytest.mark.parametrize("M", [2 ** 31 - 256, 2 ** 31 - 1, 2 ** 31])
+def test_more_grouped_rows_than_are_counted(built_library, M):
+    refused("xgen_grouped_matmul", GROUPED, dict(M=M, ar=M, N=16, G=1, ldo=16), NO, b"too many rows")
+    refused("xgen_grouped_matmul", GROUPED, dict(M=M, rows=16, N=16, G=1, ldo=16), NO, b"too many rows")

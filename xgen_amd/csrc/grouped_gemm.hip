@@ -194,7 +194,8 @@ extern "C" int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64
   if (!aligned16(bias)) return fail(XGEN_ERR_UNSUPPORTED, "%s: the bias must be 16-byte aligned", fn);
   // 32-bit offsets: within one group's weight, one tile's rows and, gathered, the whole activation
   constexpr int64_t kLimit = 0x7fffffffLL;
-  if (M > kLimit || N > kLimit / 2 || K > kLimit || ldw > 0xffffffffLL / (N + 512) || (N - 1) * ldw + K > kLimit)
+  // (rows are counted in tiles of up to 256, rounded up, in 32 bits)
+  if (M > kLimit - 256 || N > kLimit / 2 || K > kLimit || ldw > 0xffffffffLL / (N + 512) || (N - 1) * ldw + K > kLimit)
     return fail(XGEN_ERR_UNSUPPORTED, "%s: a group's weight above 2 GiB, or too many rows", fn);
   if (lda > kLimit / 512 || ldo > kLimit / 1024)
     return fail(XGEN_ERR_UNSUPPORTED, "%s: rows too long for 32-bit offsets", fn);
