@@ -533,7 +533,7 @@ int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64_t lda, int
  * weights float32, slots int32, both [tokens, k]; a negative slot adds nothing, one at or past y_rows
  * makes its row NaN.  residual: NULL or [tokens, width] of dtype; gate_table: NULL or [gate_rows, width]
  * of dtype with indices int64 [seq], tokens a multiple of seq (an index outside: a NaN row).  out [tokens, width]
- * contiguous.  width and strides multiples of 8, buffers 16-byte aligned.
+ * contiguous.  width and strides multiples of 8, buffers 16-byte aligned; k < 2^30.
  */
 int xgen_expert_combine(int dtype, const void *y, int64_t ldy, int64_t y_rows, const float *weights,
                         const int32_t *slots, int64_t tokens, int64_t k, int64_t width, const void *residual,

@@ -2,7 +2,7 @@
 call (tests/test_gpu_experts_edges.py makes the operators' calls on the device)."""
 import pytest
 
-from test_experts_cpu import BAD, GROUPED, NO, NORM, call, norm, outcome
+from test_experts_cpu import BAD, COMBINE, GROUPED, NO, NORM, call, norm, outcome
 from xgen_amd import _native as N
 
 
@@ -39,3 +39,8 @@ def test_eps_refused(built_library, eps):
 def test_more_grouped_rows_than_are_counted(built_library, M):
     refused("xgen_grouped_matmul", GROUPED, dict(M=M, ar=M, N=16, G=1, ldo=16), NO, b"too many rows")
     refused("xgen_grouped_matmul", GROUPED, dict(M=M, rows=16, N=16, G=1, ldo=16), NO, b"too many rows")
+
+
+@pytest.mark.parametrize("k", [2 ** 30, 2 ** 31 - 4, 2 ** 31 - 1, 2 ** 31])
+def test_more_choices_than_are_counted(built_library, k):
+    refused("xgen_expert_combine", COMBINE, dict(tokens=1, seq=1, k=k), NO, b"too many rows or choices")

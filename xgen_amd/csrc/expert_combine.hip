@@ -143,8 +143,9 @@ extern "C" int xgen_expert_combine(int dtype, const void *y, int64_t ldy, int64_
     return fail(XGEN_ERR_UNSUPPORTED, "%s: width and strides must be multiples of 8 elements and buffers "
                 "16-byte aligned", fn);
   const int64_t blocks = (width / 8 + 63) / 64;
-  if (width > 0x3fffffffLL || k > 0x7fffffffLL || y_rows > 0x7fffffffLL || tokens > 0x7fffffffLL / blocks)
-    return fail(XGEN_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  // (the kernel steps through the choices by four in 32 bits)
+  if (width > 0x3fffffffLL || k > 0x3fffffffLL || y_rows > 0x7fffffffLL || tokens > 0x7fffffffLL / blocks)
+    return fail(XGEN_ERR_UNSUPPORTED, "%s: too many rows or choices", fn);
   CombineArgs a;
   a.y = static_cast<const uint8_t *>(y);
   a.ldy = ldy * 2;
@@ -164,7 +165,7 @@ extern "C" int xgen_expert_combine(int dtype, const void *y, int64_t ldy, int64_
   a.indices = indices;
   a.seq = make_fastdiv((uint32_t)(gate_table ? seq : 1));
   a.out = static_cast<uint8_t *>(out);
-  const bool past = tokens * width * 2 * (k + 1 + (residual ? 1 : 0)) > kLastLevelCacheBytes;
+  const bool past = (double)tokens * width * 2 * (k + 1 + (residual ? 1 : 0)) > (double)kLastLevelCacheBytes;
   if (dtype == XGEN_DTYPE_BF16) {
     if (past) launch<XGEN_DTYPE_BF16, true>(a, stream);
     else launch<XGEN_DTYPE_BF16, false>(a, stream);
