@@ -7,6 +7,8 @@
  * arguments on the host before any HIP call and returns XGEN_OK or an error
  * code; xgen_last_error() returns a per-thread message for the last failure.
  *
+ * An output overlaps no input and no other output of its call.
+ *
  * Dtype codes (XGEN_DTYPE_*) name element types of the buffers:
  *   BF16, F16, F32 (IEEE), E4M3 (OCP float8 e4m3fn), I8, I32.
  *
@@ -486,8 +488,8 @@ int xgen_residual_norm(const void *x, int64_t x_stride_batch, int64_t x_stride_s
  * Expert router: the k experts of every token, their weights, and the grouping of the (token, choice)
  * pairs by expert that xgen_grouped_matmul and xgen_expert_combine take (no counterpart in the reference).
  * logits: [tokens, experts] of in_dtype (BF16/F16/F32), rows ld elements apart.  A token's choices are the k
- * largest of float(logit) + bias[e] (bias float32 [experts] or NULL; one fp32 addition), in descending
- * order, ties to the lowest expert; -inf and NaN are never taken.  weights float32 [tokens, k]: of the
+ * largest of float(logit) + bias[e] (bias float32 [experts] or NULL, on the logit with either scoring; one fp32
+ * addition), in descending order, ties to the lowest expert; -inf and NaN are never taken.  weights float32 [tokens, k]: of the
  * logits without bias, softmax over all experts or sigmoid, divided by their sum over the taken experts if
  * renormalize.  chosen int32 [tokens, k]: the experts.  Where fewer than k can be taken, chosen is -1 and
  * the weight 0.  A NaN logit makes its token's weights NaN.

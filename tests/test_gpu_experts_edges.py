@@ -151,3 +151,34 @@ def test_eps(cuda, eps):
     if eps in EPS_TAKEN:  # rows of zeros stay zeros
         for kind in ("rms", "layer"):
             assert not any(t.any() for t in residual_norm(z, z, norm=kind, branch_norm=kind, eps=eps))
+
+
+@pytest.mark.parametrize("scoring", [torch.sigmoid, lambda x: torch.softmax(x, 1)])
+def test_a_bias_on_the_scores(cuda, scoring):
+    """A router that ranks score + b: its biased scores as logits, its weights from the scores by the plan's experts.  By
+    logits + b the order would be another one: expert 0 has the largest bias, and a score of almost nothing."""
+    T, E, k, H = 300, 16, 4, 64
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.rand((T, E), generator=g, device=cuda) * 0.2 - 0.1
+    x[:, 0] = -40.0
+    x[7] = float("-inf")
+    b = torch.arange(E, 0, -1, device=cuda) / 4.0
+    score = scoring(x).masked_fill(x == float("-inf"), 0.0)
+    plan = route((score + b).masked_fill(x == float("-inf"), float("-inf")), k)
+    w = score.gather(1, plan.experts.long().clamp(min=0)).masked_fill(plan.experts < 0, 0)
+    w = w / w.sum(1, keepdim=True).clamp(min=torch.finfo(w.dtype).tiny)
+    live = torch.arange(T, device=cuda) != 7
+    top, order = torch.sort(scoring(x.double()) + b.double(), dim=1, descending=True)
+    assert (top[live, :k] - top[live, 1:k + 1]).min() >= 2.0 ** -20  # plain in fp32, which is off by 2^-22 at most
+    assert torch.equal(plan.experts[live].long(), order[live, :k]) and (plan.experts[live] == 0).any()
+    assert (plan.experts[7] == -1).all()
+    assert 0 not in route(x, k, bias=b, scoring="sigmoid").experts[live]
+    y = torch.randn((T * k, H), generator=g, device=cuda).bfloat16()
+    out = combine(y, w, plan.slots)
+    s = scoring(x.double()).gather(1, order[:, :k])
+    s = s / s.sum(1, keepdim=True)
+    parts = y.double()[plan.slots.long().clamp(min=0)] * s[..., None]
+    ref, mag = parts.sum(1)[live], parts.abs().sum(1)[live]
+    # a score is off by 8 * 2^-24 (an exponential, a sum of 16, a division), a weight by two of them and 4 more roundings
+    assert ((out[live].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (20 + k + 3) * 2.0 ** -24 * mag * 1.01).all()
+    assert not out[7].any()

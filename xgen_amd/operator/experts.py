@@ -55,7 +55,11 @@ def route(logits, k, *, bias=None, scoring="softmax", renormalize=True, first_ex
     """The k experts of largest logits + bias (ties to the lowest; -inf and NaN never), in that order, for logits
     BF16/F16/F32 [T, E].  Weights come from the logits without the bias: softmax over all experts, or sigmoid;
     `renormalize` divides them by their sum over the taken experts.  The plan groups the pairs of experts
-    [first_expert, first_expert + local_experts) (default: all) in the order (expert, token, choice)."""
+    [first_expert, first_expert + local_experts) (default: all) in the order (expert, token, choice).
+
+    `bias` is a prior on the logits, whatever the scoring.  A balancing bias that a router was trained with on its
+    scores (softmax(logits) + b, sigmoid(logits) + b) ranks otherwise: such a router gives its biased scores as `logits`,
+    takes the plan, and gathers its weights from the scores by `experts`."""
     _inference_only(logits, bias)
     if scoring not in _SCORINGS:
         raise ValueError(f"scoring must be one of {sorted(_SCORINGS)}")
@@ -139,8 +143,8 @@ class W8A8Experts(nn.Module):
             self.register_buffer(f"{name}_bias", bias.detach().clone() if bias is not None else None)
 
     def forward(self, x, logits, *, bias=None, residual=None, gate_table=None, indices=None):
-        """x BF16 [..., d], logits [..., E] of the router (bias: route's); the experts' sum shaped as x, or the
-        gated residual behind it (combine's)."""
+        """x BF16 [..., d], logits [..., E] of the router (bias: route's, on the logits and not on their scores); the
+        experts' sum shaped as x, or the gated residual behind it (combine's)."""
         if x.dtype != torch.bfloat16 or x.shape[-1] != self.in_features:
             raise ValueError(f"W8A8Experts requires a BF16 [..., {self.in_features}] input")
         _inference_only(x, logits)
