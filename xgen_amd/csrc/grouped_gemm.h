@@ -24,8 +24,9 @@
 //
 // Few rows are bound by the weights (8 tokens x 6 of 64 experts, 2,816 x 2,048: 35 us, 5.8 TB/s), many by the matrix
 // cores (31,248 rows of 8 experts, 14,336 x 5,376, FP8: 2.0 ms, 2.4 PFLOP/s, what one group of as many rows reaches).
-// Between them (2,049 tokens x 8 of 128 experts, 1,536 x 2,048: 105 us; without MFMAs and stores 89, without memory
-// 56) it is memory again: 504 MB read past the L2, 402 of them the weights, and 50 written, 5.3 TB/s.
+// Between them (2,049 tokens x 8 of 128 experts, 1,536 x 2,048: 105 us; with the weights read through the caches, which
+// takes as long, 89 without MFMAs and stores and 56 without memory) it is mostly memory: 449 MB read past the L2, 403 of
+// them the weights, and 57 written, 4.8 TB/s, with the matrix cores busy for 35% of the cycles.
 #pragma once
 
 #include <utility>

@@ -50,7 +50,8 @@ float above(float v, float mean, float deviation) { return 0.5f * erfcf((v - mea
 // The host does not know the groups' sizes.  They are taken to spread as a router's do: log-normal, deviation 0.4 of
 // the logarithm, and each its Poisson count.  Over those 300 calls the tile rows so come within 8% of the real
 // ones, and the choice within 1.7% of the best tile on the average (1.3% by the real ones; taking even groups
-// that end half way in a tile, 7%).
+// that end half way in a tile, 7%).  In all of them every row belongs to a group: in the plan of a rank that holds some of
+// the experts M counts rows that have no tile, and the choice is the one for that many more rows.
 float expected_tile_rows(int m, float M, float groups) {
   const float mean = M / groups;
   if (mean > 8.0f * (float)m) return M / (float)m + 0.5f * groups;
@@ -120,9 +121,12 @@ int launch(GroupedArgs g, hipStream_t stream) {
         <<<dim3((unsigned)(need < resident ? need : resident)), dim3(C::kThreads), 0, stream>>>(g);
   };
   const bool plain = g.out_dtype == XGEN_DTYPE_BF16 && g.act == XGEN_ACT_NONE;
-  // Weights that the call reads about once, in a call that passes the last-level cache, are read past the caches: 8 tokens
-  // x 6 of 64 experts, 2,816 x 2,048, 32 against 36 us; 400 tokens (37 rows an expert, 128-row tiles) 71.5 against 76.1;
-  // 1,500 (140 rows, 1.7 tile rows) 109.6 against 109.2; 31,248 rows of 8 experts 2,040 against 1,975.
+  // Weights that the call reads about once, in a call that passes the last-level cache, are read past the caches.  Both
+  // ways in turn, us past and through them, by rows an expert: 128 experts of 1,536 x 2,048 (FP8) 8 rows 65.0 / 72.4, 37
+  // 77.1 / 82.6, 60 84.1 / 86.5, 90 88.4 / 91.0, 110 101.0 / 100.8, 128 (1.45 tile rows) 108.0 / 107.7, 140 (1.56) 114.5 /
+  // 113.7, 160 119.6 / 117.0, 180 132.1 / 128.0; 64 of 2,816 x 2,048 60 rows 72.0 / 77.8, 110 88.2 / 90.3, 140 102.6 /
+  // 102.6.  Of 29 calls below the bound two lose more than 1%: 64 INT8 experts of 2,048 x 2,048 with 90 rows on 128 x 128
+  // tiles (67.0 / 64.7), 256 FP8 ones of 2,048 x 1,024 with 60 (135.0 / 130.1).
   bool once = false;
   if constexpr (C::kM <= 128) {
     const float rows = (float)g.M, groups = (float)g.groups;

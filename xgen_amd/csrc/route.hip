@@ -20,9 +20,10 @@
 //
 // A token is a group of G lanes, a lane V consecutive experts.  A choice is the maximum over the group, the lowest
 // lane that has it and that lane's lowest expert with it, which it notes in LDS: nothing but the maximum crosses
-// lanes in the loop.  What bounds it is the issue of vector instructions (1 choice 8 us, 8 choices 12) and, below,
-// the launch and two dependent reads.  15,624 tokens, 128 experts, 8 choices, bf16: 10.5 us and the placement 6.8; a
-// wave per token, a ballot per logit and the counts read one by one took 14 and 12.
+// lanes in the loop.  15,624 tokens, 128 experts, bf16: 8.2 us for one choice and 10.8 for eight, and the placement 6.8
+// (a wave per token, a ballot per logit and the counts read one by one took 14 and 12).  So a choice costs 0.4 us of
+// vector issue, and most of the time does not depend on them: 5.0 us at 501 tokens and 5.1 at 4,096 (the launch and two
+// dependent reads), 14.4 at 32,768.
 #include "xgen_common.h"
 
 namespace xgen {
