@@ -7,8 +7,6 @@
  * arguments on the host before any HIP call and returns XGEN_OK or an error
  * code; xgen_last_error() returns a per-thread message for the last failure.
  *
- * An output overlaps no input and no other output of its call.
- *
  * Dtype codes (XGEN_DTYPE_*) name element types of the buffers:
  *   BF16, F16, F32 (IEEE), E4M3 (OCP float8 e4m3fn), I8, I32.
  *
@@ -474,6 +472,7 @@ int xgen_fp8_wire_decode_strided(int out_dtype, int streams, const void *wire, i
  * (ignored for BF16).  An index outside the tables makes what its row takes from them NaN: the stream
  * if there is a gate, the rows in either case (quantized: NaN bytes or zeros, and a NaN scale).
  * width <= XGEN_NORM_MAX_WIDTH; width and strides multiples of 8, buffers 16-byte aligned; eps in [2^-126, 1).
+ * The outputs overlap no input.
  */
 int xgen_residual_norm(const void *x, int64_t x_stride_batch, int64_t x_stride_seq, const void *branch,
                        int64_t br_stride_batch, int64_t br_stride_seq, int64_t batch, int64_t seq, int64_t width,
@@ -520,6 +519,7 @@ int xgen_route(int in_dtype, const void *logits, int64_t ld, int64_t tokens, int
  * (one scale, or a_rows); w_scale_stride 0 ([groups]) or 1 ([groups, N]).  bias: NULL or [groups, N].
  * out [M, N], rows ldo apart.  K, N multiples of 16, rows and the bias 16-byte aligned; one group's weight below
  * 2 GiB, and with rows the activation too; M < 2^31 - 256; groups <= XGEN_ROUTE_MAX_EXPERTS.
+ * out overlaps no operand.
  */
 int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64_t lda, int64_t a_rows, const void *w,
                         int64_t ldw, int64_t w_group_stride, int64_t M, int64_t N, int64_t K, int64_t groups,
@@ -535,7 +535,7 @@ int xgen_grouped_matmul(int in_dtype, int exact, const void *a, int64_t lda, int
  * weights float32, slots int32, both [tokens, k]; a negative slot adds nothing, one at or past y_rows
  * makes its row NaN.  residual: NULL or [tokens, width] of dtype; gate_table: NULL or [gate_rows, width]
  * of dtype with indices int64 [seq], tokens a multiple of seq (an index outside: a NaN row).  out [tokens, width]
- * contiguous.  width and strides multiples of 8, buffers 16-byte aligned; k < 2^30.
+ * contiguous.  width and strides multiples of 8, buffers 16-byte aligned; k < 2^30.  out does not overlap y.
  */
 int xgen_expert_combine(int dtype, const void *y, int64_t ldy, int64_t y_rows, const float *weights,
                         const int32_t *slots, int64_t tokens, int64_t k, int64_t width, const void *residual,
