@@ -29,7 +29,8 @@ extern "C" {
 
 /* raised when an entry point changes or goes; a library from before one was added has the same
  * version and lacks the symbol (since version 1: xgen_fp8_quantize_tensor, xgen_residual_norm, xgen_route,
- * xgen_route_workspace_bytes, xgen_grouped_matmul, xgen_expert_combine) */
+ * xgen_route_workspace_bytes, xgen_grouped_matmul, xgen_expert_combine, xgen_mxfp4_quantize, xgen_mxfp4_dequantize,
+ * xgen_mxfp4_matmul, xgen_qk_norm_rope, xgen_rotary_table) */
 #define XGEN_ABI_VERSION 1
 
 /* status codes */
@@ -54,7 +55,7 @@ extern "C" {
 #define XGEN_WIRE_MAX_WIDTH 1024
 
 /* normalisation kinds for xgen_norm_affine_quant and xgen_residual_norm */
-#define XGEN_NORM_NONE (-1) /* xgen_residual_norm: the branch as it is */
+#define XGEN_NORM_NONE (-1) /* xgen_residual_norm, xgen_qk_norm_rope: the values as they are */
 #define XGEN_NORM_LAYER 0 /* (x - mean) * rsqrt(var + eps), biased variance */
 #define XGEN_NORM_RMS 1   /* x * rsqrt(mean(x^2) + eps) */
 /* OR-ed into norm_kind: scale_table holds bf16(1 + scale) (xgen_adaln_one_plus) */
@@ -69,6 +70,13 @@ extern "C" {
 #define XGEN_ROUTE_SIGMOID 1
 #define XGEN_ROUTE_MAX_EXPERTS 512
 #define XGEN_ROUTE_MAX_CHOICES 32
+
+/* MXFP4 scales: the power of two below a block's largest value over 4, or the least that saturates none */
+#define XGEN_MX_FLOOR 0
+#define XGEN_MX_CEIL 1
+
+/* widest head of xgen_qk_norm_rope */
+#define XGEN_HEAD_MAX_DIM 512
 
 /* Largest row width of the fused norm kernel (the reference limit,
  * x_base/x_base/operator/npu_fusion/capabilities.py:7, is 6144). */
@@ -541,6 +549,66 @@ int xgen_expert_combine(int dtype, const void *y, int64_t ldy, int64_t y_rows, c
                         const int32_t *slots, int64_t tokens, int64_t k, int64_t width, const void *residual,
                         int64_t ld_residual, const void *gate_table, int64_t gate_row_stride, int64_t gate_rows,
                         const int64_t *indices, int64_t seq, void *out, hipStream_t stream);
+
+/*
+ * MXFP4 rows: e2m1 codes, two per byte (the value of even k in the low four bits), with one power-of-two scale
+ * (e8m0, byte E + 127) per 32 consecutive values of a row (the OCP microscaling format; no counterpart in the
+ * reference).  Quantize: E = floor(log2 max|x|) - 2 (XGEN_MX_FLOOR, the format's rule: values between 6 and 8 times
+ * 2^E saturate) or the least E with max|x| <= 6 * 2^E (XGEN_MX_CEIL), at least -127; code = x / 2^E to nearest, ties to the
+ * even code, saturated at 6.  A block with an inf or NaN: scale byte 255 (NaN), codes 0.  Dequantize:
+ * out = code * 2^E rounded to out_dtype (BF16, F16 or F32; exact in BF16 for what was quantized, F32), NaN where the scale is 255.
+ * Dense rows: [rows, K], ld elements apart; codes: [rows, K / 2] bytes, ld_codes bytes apart; scales:
+ * [(K + 255) / 256][rows + rows % 2][8] bytes, block_stride bytes between two blocks of 256 values, whose eight bytes
+ * of a row hold its block i of 32 at (i % 2) * 4 + i / 2.  Quantize writes all of them (zeros for the blocks past K and the row that makes
+ * the number even).  K a multiple of 32; dense rows, codes and scale blocks 16-byte aligned.  The outputs overlap no input.
+ */
+int xgen_mxfp4_quantize(int in_dtype, const void *x, int64_t rows, int64_t K, int64_t ldx, int rounding, void *codes,
+                        int64_t ld_codes, void *scales, int64_t block_stride, hipStream_t stream);
+int xgen_mxfp4_dequantize(const void *codes, int64_t ld_codes, const void *scales, int64_t block_stride, int64_t rows,
+                          int64_t K, int out_dtype, void *out, int64_t ldo, hipStream_t stream);
+
+/*
+ * Product of MXFP4 rows, as xgen_scaled_mm_fp8 of 8-bit ones (no counterpart in the reference):
+ *   y[m, n] = sum_k a[m, k] * w[n, k] + bias[n], summed in fp32;  out = out_dtype(y),
+ *   out_dtype(gelu_tanh(out_dtype(y))) with XGEN_ACT_GELU_TANH, or with a residual (BF16, no activation)
+ *   bf16(residual[m] + bf16(bf16(y) * gate_table[indices[m % seq]])), the roundings of xgen_w8a8_gate_residual.
+ * a [M, K], w [N, K]: codes and scales as xgen_mxfp4_quantize lays them out (lda, ldw and block strides in bytes).
+ * A row or weight row with a scale of 255 gives NaN.  bias: NULL or [N] of BF16, F16 or F32.  residual NULL or BF16
+ * [M, N]; gate_table BF16 [gate_rows, N] with indices int64 [seq], M a multiple of seq (an index outside: a NaN row).
+ * K a multiple of 32, N of 16; rows, bias and scale blocks 16-byte aligned; w below 2 GiB.  out overlaps no operand.
+ */
+int xgen_mxfp4_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_block_stride, const void *w,
+                      int64_t ldw, const void *w_scales, int64_t w_block_stride, int64_t M, int64_t N, int64_t K,
+                      const void *bias, int bias_dtype, int activation, const void *residual, int64_t ld_residual,
+                      const void *gate_table, int64_t gate_row_stride, int64_t gate_rows, const int64_t *indices,
+                      int64_t seq, void *out, int out_dtype, int64_t ldo, hipStream_t stream);
+
+/*
+ * The norms of queries and keys over each head and their position rotation in one pass (no counterpart in the
+ * reference, whose path ends at the projections):
+ *   v = norm(x) * weight over a head's dim values;  of its first 2 * pairs values, (i, i + pairs) or with `interleaved`
+ *   (2 i, 2 i + 1) are a pair (a, b):  out = (a cos[p, i] - b sin[p, i], b cos[p, i] + a sin[p, i]);  the others: v
+ * in fp32, rounded once.  q [batch, seq, q_heads, dim], k [batch, seq, k_heads, dim] of dtype (BF16/F16), strides in elements,
+ * last stride 1 (views of a fused projection's rows; either may have no heads); q_out, k_out contiguous of the same
+ * shapes.  norm_kind XGEN_NORM_NONE (no weights), _LAYER or _RMS; weights NULL or [dim] of weight_dtype (BF16/F16/F32).
+ * cos, sin: float32 [places, pairs] (xgen_rotary_table's).  p = positions[b * position_stride_batch + s], or s if positions is
+ * NULL; a position outside [0, places) makes its token's heads NaN.  dim a multiple of 8, up to XGEN_HEAD_MAX_DIM; strides
+ * multiples of 8, heads 16-byte aligned; eps in [2^-126, 1).  The outputs overlap no input.
+ */
+int xgen_qk_norm_rope(int dtype, const void *q, int64_t q_stride_batch, int64_t q_stride_seq, int64_t q_stride_head,
+                      int64_t q_heads, const void *k, int64_t k_stride_batch, int64_t k_stride_seq,
+                      int64_t k_stride_head, int64_t k_heads, int64_t batch, int64_t seq, int64_t dim, int norm_kind,
+                      const void *q_weight, const void *k_weight, int weight_dtype, float eps, const float *cos,
+                      const float *sin, int64_t places, int64_t pairs, int interleaved, const int64_t *positions,
+                      int64_t position_stride_batch, void *q_out, void *k_out, hipStream_t stream);
+
+/*
+ * cos[p, i] = factor * cos(positions[p, axis[i]] * frequencies[i]) and sin alike, float32 [places, pairs], the
+ * angle in 64 bits (no counterpart in the reference).  positions int64 [places, axes]; frequencies float64 [pairs];
+ * axis int32 [pairs] or NULL (the first axis).  An axis outside, or an angle of 2^36 or more: NaN.
+ */
+int xgen_rotary_table(const int64_t *positions, int64_t places, int64_t axes, const double *frequencies,
+                      const int32_t *axis, int64_t pairs, double factor, float *cos, float *sin, hipStream_t stream);
 
 #ifdef __cplusplus
 }

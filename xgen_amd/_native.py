@@ -23,6 +23,7 @@ DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_E4M3, DTYPE_I8, DTYPE_I32, DTYPE_NONE = 
 NORM_LAYER, NORM_RMS, NORM_SCALE_ONE_PLUS, NORM_NONE = 0, 1, 0x100, -1
 ACT_NONE, ACT_GELU_TANH = 0, 1
 ROUTE_SOFTMAX, ROUTE_SIGMOID, ROUTE_MAX_EXPERTS, ROUTE_MAX_CHOICES = 0, 1, 512, 32
+MX_FLOOR, MX_CEIL, HEAD_MAX_DIM = 0, 1, 512
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 
 _TORCH_DTYPE = {
@@ -113,12 +114,24 @@ SIGNATURES = {
     "xgen_expert_combine": (_c_int, [
         _c_int, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64,
         _c_ptr, _c_i64, _c_ptr, _c_ptr]),
+    "xgen_mxfp4_quantize": (_c_int, [_c_int, _c_ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr]),
+    "xgen_mxfp4_dequantize": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_i64, _c_ptr]),
+    "xgen_mxfp4_matmul": (_c_int, [
+        _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int,
+        _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_int, _c_i64, _c_ptr]),
+    "xgen_qk_norm_rope": (_c_int, [
+        _c_int, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+        _c_int, _c_ptr, _c_ptr, _c_int, _c_float, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_int, _c_ptr, _c_i64, _c_ptr, _c_ptr,
+        _c_ptr]),
+    "xgen_rotary_table": (_c_int, [
+        _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, ctypes.c_double, _c_ptr, _c_ptr, _c_ptr]),
 }
 
 
 # added within ABI version 1: a library from before them still loads
 ADDED = frozenset({"xgen_fp8_quantize_tensor", "xgen_residual_norm", "xgen_route", "xgen_route_workspace_bytes",
-                   "xgen_grouped_matmul", "xgen_expert_combine"})
+                   "xgen_grouped_matmul", "xgen_expert_combine", "xgen_mxfp4_quantize", "xgen_mxfp4_dequantize",
+                   "xgen_mxfp4_matmul", "xgen_qk_norm_rope", "xgen_rotary_table"})
 
 
 def library_path() -> Path:

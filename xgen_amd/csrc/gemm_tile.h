@@ -1,4 +1,4 @@
-// The W8A8 GEMM on tiles below 256 x 256 (gfx950): one output tile per
+// The W8A8 and MXFP4 GEMM on tiles below 256 x 256 (gfx950): one output tile per
 // workgroup, for calls whose 256 x 256 tiles would leave compute units idle.
 //
 // A workgroup of WM x WN waves computes a (32 WM FM) x (32 WN FN) output tile;
@@ -56,6 +56,12 @@ struct TileCfg {
   static_assert(kM % (8 * kWaves) == 0 && kN % (8 * kWaves) == 0 && kM <= 256 && kN <= 256, "DMA split");
   static_assert((SLOTS - 1) * kLoads < 64, "vmcnt range");
   static_assert(kLdsBytes <= 160 * 1024, "LDS");
+  // MXFP4: the scale bytes of a pair, 8 of a row, in their own ring: one 1 KB load (128 rows of one operand) per wave,
+  // the first waves' the activations, the next ones' the weights, the rest's of nothing
+  static constexpr int kScaleA = (kM + 127) / 128, kScaleW = (kN + 127) / 128;
+  static constexpr int kScaleSlot = kWaves * 1024, kScaleBase = kLdsBytes;
+  static constexpr int kMxLdsBytes = kScaleBase + SLOTS * kScaleSlot;
+  static_assert(kScaleA + kScaleW <= kWaves && kMxLdsBytes <= 160 * 1024, "scales");
 };
 
 template <int KIND, int WM, int WN, int FM, int FN, int SLOTS, bool GATED>
@@ -65,6 +71,8 @@ void gemm_tile_kernel(GemmArgs p) {
   typedef Mfma<KIND> T;
   typedef typename T::frag_t frag_t;
   constexpr int KS = T::kSteps;
+  constexpr bool kMx = KIND == kMx4;
+  constexpr int kPairLoads = C::kLoads + (kMx ? 1 : 0);  // per wave
   constexpr int kMfmas = KS * FM * FN;     // per sub-stage per wave (64-byte steps of the exact kind count once)
   // three slots or more: a pair's DMA loads are spread over two sub-stages (all in one queue
   // up in the address unit ahead of the MFMAs: 3% to 11% slower)
@@ -73,7 +81,7 @@ void gemm_tile_kernel(GemmArgs p) {
   // fit the registers widened
   constexpr bool kWeightsOuter = FM <= 2;
   constexpr int kFrags = KS * (FM + FN);   // fragment reads per sub-stage per wave
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[C::kLdsBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kMx ? C::kMxLdsBytes : C::kLdsBytes];
 
   // --- this workgroup's tile: consecutive workgroup ids go to the 8 XCDs round-robin,
   // XCD x owns a contiguous range of tiles ---
@@ -95,7 +103,7 @@ void gemm_tile_kernel(GemmArgs p) {
   // from here to the epilogue, which shares them through LDS ---
   static_assert(C::kM <= C::kThreads && C::kN <= C::kThreads, "one token and one feature per thread");
   const int pm = min(m0 + tid, p.M - 1), pn = min(n0 + tid, p.N - 1);
-  const float sa_t = p.sa[p.sa_stride ? pm : 0], sw_t = p.sw[p.sw_stride ? pn : 0];
+  const float sa_t = kMx ? 1.0f : p.sa[p.sa_stride ? pm : 0], sw_t = kMx ? 1.0f : p.sw[p.sw_stride ? pn : 0];
   float bias_t = 0.0f;
   if (p.bias) {  // uniform
     if (p.bias_dtype == XGEN_DTYPE_F32) bias_t = static_cast<const float *>(p.bias)[pn];
@@ -114,7 +122,21 @@ void gemm_tile_kernel(GemmArgs p) {
   uint32_t dma_slot = 0;     // its slot's LDS offset
   uint32_t oa = 0, ow = 0;   // its offsets, or out of range
   // (kOutOfRange + rows * ld stays out of range: the host keeps (M + 512) * lda below 2^32)
+  [[maybe_unused]] uint32_t scale_slot = 0;  // MXFP4: dma_slot's place in the scales' ring
   auto issue_begin = [&]() {
+    if constexpr (kMx) {
+      // a resource of one 256-value block's rows, empty past K and for waves without a share (zeros)
+      const bool act = wave < C::kScaleA;
+      const int first = act ? m0 : n0, part = act ? wave : wave - C::kScaleA, rows = act ? C::kM : C::kN;
+      const int64_t block = dma_k >> 7;
+      const bool some = dma_k < p.K && wave < C::kScaleA + C::kScaleW;
+      const __amdgpu_buffer_rsrc_t rs =
+          rsrc(act ? p.xs + block * p.xs_block : p.ws + block * p.ws_block, some ? (act ? p.xs_rows : p.ws_rows) : 0);
+      const int row = part * 128 + lane * 2;
+      dma_load16(rs, smem + C::kScaleBase + scale_slot + wave * 1024,
+                 row < rows ? (uint32_t)(first + row) * 8 : kOutOfRange);
+      scale_slot = scale_slot + C::kScaleSlot == SLOTS * C::kScaleSlot ? 0 : scale_slot + C::kScaleSlot;
+    }
     const bool live = dma_k + ch < p.K;
     oa = live ? offa + dma_k : kOutOfRange;
     ow = live ? offw + dma_k : kOutOfRange;
@@ -136,9 +158,18 @@ void gemm_tile_kernel(GemmArgs p) {
   // --- fragments: [register buffer = sub-stage][k step][fragment] ---
   const int row_x = wm * 32 * FM + (lane & 31), row_w = wn * 32 * FN + (lane & 31);
   frag_t xf[2][KS][FM], wf[2][KS][FN];
+  [[maybe_unused]] uint32_t xsc[2][kMx ? FM : 1], wsc[2][kMx ? FN : 1];
   uint32_t rd_slot = 0;  // LDS offset of the pair being multiplied
-  auto read_frag = [&](int b, uint32_t slot, int r) {  // fragment r of sub-stage b, weights first
+  // fragment r of sub-stage b, weights first (sslot: the slot's place in the scales' ring)
+  auto read_frag = [&](int b, uint32_t slot, [[maybe_unused]] uint32_t sslot, int r) {
     const int ks = r / (FM + FN), f = r % (FM + FN);
+    if constexpr (kMx) {  // with step 0's fragment, the row's two scale bytes of the sub-stage
+      if (ks == 0) {
+        const uint32_t sc = C::kScaleBase + sslot + (lane >> 5) * 4 + b * 2;
+        if (f < FN) wsc[b][f] = *reinterpret_cast<const uint16_t *>(smem + sc + C::kScaleA * 1024 + (row_w + f * 32) * 8);
+        else xsc[b][f - FN] = *reinterpret_cast<const uint16_t *>(smem + sc + (row_x + (f - FN) * 32) * 8);
+      }
+    }
     if (f < FN) wf[b][ks][f] = load_pair<KIND>(smem + slot + C::kM * 128, row_w + f * 32, b, ks, lane);
     else xf[b][ks][f - FN] = load_pair<KIND>(smem + slot, row_x + (f - FN) * 32, b, ks, lane);
   };
@@ -158,6 +189,7 @@ void gemm_tile_kernel(GemmArgs p) {
     constexpr int b = decltype(B)::value;
     constexpr bool load = decltype(LOAD)::value, read = decltype(READ)::value;
     if constexpr (b == 1 && load) issue_begin();
+    const uint32_t next_sslot = kMx ? next_slot / C::kSlotBytes * C::kScaleSlot : 0;
     // the MFMAs are volatile asm statements: the loads written between them stay there
     // (the exact kind widens each activation fragment once per sub-stage and, weights
     // outermost, each weight fragment once too)
@@ -174,6 +206,10 @@ void gemm_tile_kernel(GemmArgs p) {
         const int j = s / FN, i = s % FN;
         if (i == 0) xw[0] = MfmaA<KIND>::widen_x(xf[b][ks][j]);
         MfmaA<KIND>::mma(acc[i][j], wf[b][ks][i], xw[0]);
+      } else if constexpr (kMx) {
+        const int j = (s / FN) % FM, i = s % FN;
+        if (ks == 0) MfmaA<KIND>::template mma<0>(acc[i][j], wf[b][ks][i], xf[b][ks][j], wsc[b][i], xsc[b][j]);
+        else MfmaA<KIND>::template mma<1>(acc[i][j], wf[b][ks][i], xf[b][ks][j], wsc[b][i], xsc[b][j]);
       } else {
         const int j = (s / FN) % FM, i = s % FN;
         MfmaA<KIND>::mma(acc[i][j], wf[b][ks][i], xf[b][ks][j]);
@@ -181,7 +217,7 @@ void gemm_tile_kernel(GemmArgs p) {
       if constexpr (read) {
 #pragma unroll
         for (int r = spread_first(s, kFrags, kMfmas); r < spread_first(s + 1, kFrags, kMfmas); ++r)
-          read_frag(b ^ 1, next_slot, r);
+          read_frag(b ^ 1, next_slot, next_sslot, r);
       }
       if constexpr (load && kSpread) {
         // sub-stage 1 takes the first half of a pair's loads, the next sub-stage 0 the rest
@@ -208,17 +244,17 @@ void gemm_tile_kernel(GemmArgs p) {
     for (int q = 0; q < (kSpread && s == SLOTS - 1 ? (C::kLoads + 1) / 2 : C::kLoads); ++q) issue_load(q);
     if (!(kSpread && s == SLOTS - 1)) issue_end();
   }
-  wait_vmcnt<(SLOTS - 1) * C::kLoads - (kSpread ? C::kLoads / 2 : 0)>();
+  wait_vmcnt<(SLOTS - 1) * kPairLoads - (kSpread ? C::kLoads / 2 : 0)>();
   lds_barrier();
 #pragma unroll
-  for (int r = 0; r < kFrags; ++r) read_frag(0, 0, r);
+  for (int r = 0; r < kFrags; ++r) read_frag(0, 0, 0, r);
 
   // pairs past K are zeros: the ring is filled once at least
   const int pairs = (p.K + 127) / 128 > SLOTS ? (p.K + 127) / 128 : SLOTS;
   // waits for this thread's loads of the next pair (`newer` pairs were issued after them),
   // then publishes every wave's and retires the reads of this one
   auto publish = [&](auto NEWER) {
-    wait_vmcnt<decltype(NEWER)::value * C::kLoads>();
+    wait_vmcnt<decltype(NEWER)::value * kPairLoads>();
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     lds_barrier();
   };

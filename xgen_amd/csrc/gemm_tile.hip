@@ -1,4 +1,4 @@
-// Choice and launch of the W8A8 GEMM's smaller tiles (gemm_tile.h).
+// Choice and launch of the W8A8 and MXFP4 GEMM's smaller tiles (gemm_tile.h).
 #include "gemm_tile.h"
 
 namespace xgen {
@@ -40,7 +40,7 @@ constexpr TileSize kTileSizes[kTiles + 1] = {XGEN_GEMM_TILES(XGEN_TILE_SIZE){kTi
 struct TileCost {
   float per_pair, per_tile, start;
 };
-constexpr TileCost kTileCosts[3][kTiles + 1] = {
+constexpr TileCost kTileCosts[4][kTiles + 1] = {
     // INT8
     {{0.203f, 0.1f, 3.1f}, {0.319f, 0.0f, 3.7f}, {0.242f, 2.1f, 1.3f}, {0.39f, 1.3f, 3.3f}, {0.503f, 3.9f, 1.8f},
      {0.668f, 5.2f, 1.8f}, {0.751f, 7.3f, 0.0f}, {1.18f, 8.5f, 0.0f}, {1.54f, 6.7f, 0.1f}},
@@ -50,6 +50,9 @@ constexpr TileCost kTileCosts[3][kTiles + 1] = {
     // FP8 exact
     {{0.266f, 0.0f, 4.0f}, {0.363f, 0.0f, 3.9f}, {0.367f, 2.2f, 1.5f}, {0.492f, 3.0f, 1.2f}, {0.771f, 4.7f, 0.0f},
      {1.06f, 4.8f, 0.0f}, {1.35f, 6.4f, 0.0f}, {1.92f, 7.8f, 0.0f}, {2.49f, 7.7f, 0.0f}},
+    // MXFP4
+    {{0.203f, 0.1f, 3.1f}, {0.319f, 0.0f, 3.7f}, {0.242f, 2.1f, 1.3f}, {0.39f, 1.3f, 3.3f}, {0.503f, 3.9f, 1.8f},
+     {0.668f, 5.2f, 1.8f}, {0.751f, 7.3f, 0.0f}, {1.18f, 8.5f, 0.0f}, {1.54f, 6.7f, 0.1f}},
 };
 // The 256 x 256 kernel keeps a call unless a smaller tile is put 4% below it.  On short K, where
 // the sums put its epilogue too high, 10%: up to K = 512, and against the tiles from 128 x 192 on up
@@ -120,7 +123,8 @@ int choose_gemm_tile(int kind, int64_t M, int64_t N, int64_t K, bool gated, bool
 void launch_gemm_tile(int kind, int tile, const GemmArgs &g, hipStream_t stream) {
   if (kind == kInt8) launch_kind<kInt8>(tile, g, stream);
   else if (kind == kFp8) launch_kind<kFp8>(tile, g, stream);
-  else launch_kind<kFp8Exact>(tile, g, stream);
+  else if (kind == kFp8Exact) launch_kind<kFp8Exact>(tile, g, stream);
+  else launch_kind<kMx4>(tile, g, stream);
 }
 
 }  // namespace xgen

@@ -1,4 +1,4 @@
-// Pieces shared by the W8A8 GEMM kernels (gemm_w8a8.hip: one persistent workgroup
+// Pieces shared by the W8A8 and MXFP4 GEMM kernels (gemm_w8a8.hip: one persistent workgroup
 // per CU on 256 x 256 tiles; gemm_tile.hip: smaller tiles): the arguments, the
 // operand kinds' MFMA wrappers, the LDS-DMA load and the LDS row layout.
 #pragma once
@@ -41,6 +41,11 @@ struct GemmArgs {
   const int64_t *indices;
   uint32_t seq, seq_magic, seq_shift;  // m % seq = m - ((mulhi(m, magic) + m) >> shift) * seq
   uint32_t residual_bytes, gate_bytes;  // (M - 1) * ld_residual * 2 + N * 2, (gate_rows - 1) * gate_stride * 2 + N * 2
+  // scale bytes of 32 values (kMx4 only): 8 bytes per row and 256 values, xs_block / ws_block bytes between two
+  // such blocks of all rows; bytes of one block's rows (an even number of them)
+  const uint8_t *xs, *ws;
+  int64_t xs_block, ws_block;
+  uint32_t xs_rows, ws_rows;
 };
 
 // A grouped call's arguments (grouped_gemm.hip): M is the rows of all groups, N, K and the strides are every
@@ -55,7 +60,7 @@ struct GroupedArgs : GemmArgs {
 };
 
 // Operand kinds of the kernel template.
-enum Kind { kInt8 = 0, kFp8 = 1, kFp8Exact = 2 };
+enum Kind { kInt8 = 0, kFp8 = 1, kFp8Exact = 2, kMx4 = 3 };  // (K, lda and ldw of kMx4: bytes, two values each)
 
 // The smaller tile that a call runs on, or -1: the 256 x 256 kernel (gemm_tile.hip).
 int choose_gemm_tile(int kind, int64_t M, int64_t N, int64_t K, bool gated, bool accumulators);
@@ -102,6 +107,18 @@ struct Mfma<kInt8> {
   static constexpr int kSteps = BK / 32;  // 32x32x32: two steps per stage
   static constexpr int kReads = 1;        // ds_read_b128 per fragment
   static __device__ __forceinline__ float to_f32(int v) { return (float)v; }
+};
+
+// MXFP4: fragments lie as INT8's.  Lane half h of a 32x32x64 step holds one block of 32 values per row, and a row's
+// 8 scale bytes of 256 values are ordered (block mod 2) * 4 + block / 2: a lane's four bytes of a pair (its
+// blocks h, h + 2, h + 4, h + 6) are one dword, step s taking byte s.
+template <>
+struct Mfma<kMx4> {
+  typedef f32x16 acc_t;
+  typedef i32x4 frag_t;
+  static constexpr int kSteps = BK / 32;  // 32x32x64 of half a byte: two steps per stage
+  static constexpr int kReads = 1;        // ds_read_b128 per fragment
+  static __device__ __forceinline__ float to_f32(float v) { return v; }
 };
 
 // One 16-byte-per-lane buffer load on the LDS-DMA path: lane l's 16 bytes land
@@ -198,6 +215,24 @@ struct MfmaA<kInt8> {
     asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, 0" : "=a"(c) : "v"(w), "v"(x));
   }
 };
+// BYTE: the byte of both scale dwords that holds this step's block.
+template <>
+struct MfmaA<kMx4> {
+#define XGEN_MX4(ADDEND, OPSEL) "v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, " ADDEND ", %3, %4 " OPSEL " cbsz:4 blgp:4"
+  template <int BYTE>
+  static __device__ __forceinline__ void mma(f32x16 &c, const i32x4 &w, const i32x4 &x, uint32_t sw, uint32_t sx) {
+    static_assert(BYTE >= 0 && BYTE < 4, "scale byte");
+    if constexpr (BYTE == 0) asm volatile(XGEN_MX4("%0", "op_sel_hi:[0,0,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+    else if constexpr (BYTE == 1) asm volatile(XGEN_MX4("%0", "op_sel:[1,1,0] op_sel_hi:[0,0,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+    else if constexpr (BYTE == 2) asm volatile(XGEN_MX4("%0", "op_sel_hi:[1,1,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+    else asm volatile(XGEN_MX4("%0", "op_sel:[1,1,0] op_sel_hi:[1,1,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+  }
+  // (a tile's first step is byte 0's)
+  static __device__ __forceinline__ void mma0(f32x16 &c, const i32x4 &w, const i32x4 &x, uint32_t sw, uint32_t sx) {
+    asm volatile(XGEN_MX4("0", "op_sel_hi:[0,0,0]") : "=a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+  }
+#undef XGEN_MX4
+};
 // The exact kind: e4m3fn fragments in the FP8 kind's layout, widened to bf16
 // (exact for every code) and multiplied by four 32x32x16 bf16 MFMAs, step s on
 // bytes 8s..8s+7 of each lane's 32 from both operands, so every product pairs
@@ -250,7 +285,7 @@ struct MfmaA<kFp8Exact> {
 __device__ __forceinline__ int swz128(int row, int chunk) { return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4); }
 template <int KIND>
 __device__ __forceinline__ typename Mfma<KIND>::frag_t load_pair(const uint8_t *tile, int row, int half, int ks, int lane) {
-  if constexpr (KIND == kInt8) {
+  if constexpr (KIND == kInt8 || KIND == kMx4) {
     const u32x4 v = *reinterpret_cast<const u32x4 *>(tile + swz128(row, half * 4 + ks * 2 + (lane >> 5)));
     return typename Mfma<KIND>::frag_t{(int)v.x, (int)v.y, (int)v.z, (int)v.w};
   } else {

@@ -10,6 +10,8 @@
 //              matrix-core time of the FP8 instructions, plus the conversions
 //   INT8     : v_mfma_i32_32x32x32_i8      (int8 x int8 -> exact int32)
 //              replaces torch_npu.npu_quant_matmul at x_base/x_base/operator/matmul.py:63-64
+//   MXFP4    : v_mfma_scale_f32_32x32x64_f8f6f4 (e2m1 x e2m1, one e8m0 scale per 32
+//              values of either operand -> fp32), in its own entry (xgen_mxfp4_matmul)
 //
 // The FP8 instructions (all shapes, measured on gfx950) do not sum like IEEE
 // fp32: within each group of 8 consecutive K the products are truncated toward
@@ -94,6 +96,19 @@ constexpr int kXposeRow = 136;
 constexpr int kXpose = 32 * kXposeRow;
 constexpr int kXposeBase = kParamBase + kParamSets * kParamBytes;
 constexpr int kLdsBytes = kXposeBase + kWaves * kXpose;  // 154 KB
+// MXFP4: a parameter set is its bias row, and behind the transpose areas each pair slot has the scale bytes of
+// its 256 activation and 256 weight rows, 8 of a row.  One 1 KB load per wave and pair: waves 0 and 1 the
+// activations' halves, 2 and 3 the weights'.
+constexpr int kScaleSlot = 2 * 256 * 8;
+template <int KIND>
+struct Lds {
+  static constexpr bool kMx = KIND == kMx4;
+  static constexpr int kParam = kMx ? 1024 : kParamBytes, kBias = kMx ? 0 : 2048;
+  static constexpr int kXpose0 = kParamBase + kParamSets * kParam;
+  static constexpr int kScale0 = kXpose0 + kWaves * kXpose;
+  static constexpr int kBytes = kScale0 + (kMx ? kPairSlots * kScaleSlot : 0);
+  static_assert(kBytes <= 160 * 1024 && (kMx || kBytes == kLdsBytes), "LDS");
+};
 }  // namespace w4
 
 // 24 wait states after the last MFMAs before any accumulator is read by VALU
@@ -117,7 +132,9 @@ void gemm_w4_kernel(GemmArgs p) {
   constexpr int FM = 4, FN = 4, KS = T::kSteps;
   constexpr int kMfmas = KS * FM * FN;                 // per stage per wave
   constexpr int kReads = T::kReads * KS * (FM + FN);   // ds_read_b128 per stage per wave
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kLdsBytes];
+  typedef Lds<KIND> L;
+  constexpr bool kMx = KIND == kMx4;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[L::kBytes];
 
   // --- this workgroup's tiles: a contiguous range per XCD, strided by workgroup ---
   const int ntiles = p.tiles_m * p.tiles_n;
@@ -143,8 +160,8 @@ void gemm_w4_kernel(GemmArgs p) {
       const_cast<float *>(p.sw), (short)0, p.N * 4, kBufferFlags);
   const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<void *>(p.bias), (short)0, p.bias ? p.N * bias_elem : 0, kBufferFlags);
-  const float sa0 = p.sa_stride ? 0.0f : p.sa[0];  // per-tensor scales
-  const float sw0 = p.sw_stride ? 0.0f : p.sw[0];
+  const float sa0 = kMx || p.sa_stride ? 0.0f : p.sa[0];  // per-tensor scales
+  const float sw0 = kMx || p.sw_stride ? 0.0f : p.sw[0];
   // the output rows as a buffer: stores at kOutOfRange are dropped
   const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(p.out, (short)0, (int)p.out_bytes, kBufferFlags);
   // the gated epilogue's residual rows and gate table (reads past them return zeros)
@@ -178,11 +195,24 @@ void gemm_w4_kernel(GemmArgs p) {
   };
   auto issue_begin = [&](int slot) {
     if (dma_k == 0 && dma_h < GP) {  // the tile's epilogue parameters ride with its first pair
-      uint8_t *prm = smem + kParamBase + (dma_i % kParamSets) * kParamBytes;
-      if (wave == 0 && p.sa_stride) dma_load16(rsa, prm, (uint32_t)dma_m0 * 4 + lane * 16);
-      if (wave == 1 && p.sw_stride) dma_load16(rsw, prm + 1024, (uint32_t)dma_n0 * 4 + lane * 16);
+      uint8_t *prm = smem + kParamBase + (dma_i % kParamSets) * L::kParam;
+      if constexpr (!kMx) {
+        if (wave == 0 && p.sa_stride) dma_load16(rsa, prm, (uint32_t)dma_m0 * 4 + lane * 16);
+        if (wave == 1 && p.sw_stride) dma_load16(rsw, prm + 1024, (uint32_t)dma_n0 * 4 + lane * 16);
+      }
       // (without a bias the resource is empty: the row reads as zeros)
-      if (wave == 2) dma_load16(rb, prm + 2048, (uint32_t)(dma_n0 * bias_elem) + lane * 16);
+      if (wave == 2) dma_load16(rb, prm + L::kBias, (uint32_t)(dma_n0 * bias_elem) + lane * 16);
+    }
+    if constexpr (kMx) {
+      // the pair's scale bytes: a resource of one 256-value block's rows, empty past K (zeros: 2^-127 times
+      // the zero codes there)
+      const bool act = wave < 2;
+      const bool some = dma_h < GP && dma_k * 128 < p.K;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t *>(act ? p.xs + dma_k * p.xs_block : p.ws + dma_k * p.ws_block), (short)0,
+          some ? (int)(act ? p.xs_rows : p.ws_rows) : 0, kBufferFlags);
+      dma_load16(rs, smem + L::kScale0 + slot * kScaleSlot + wave * 1024,
+                 (uint32_t)((act ? dma_m0 : dma_n0) + (wave & 1) * 128) * 8 + lane * 16);
     }
     const int k0 = dma_k * 128;
     const bool live = dma_h < GP;
@@ -222,6 +252,14 @@ void gemm_w4_kernel(GemmArgs p) {
     wf[b][ks][i] = load_pair<KIND>(smem + (s >> 1) * kPairSlotBytes + kPairTile, row_w + i * 32, s & 1, ks, lane);
   };
 
+  // MXFP4: this lane's four scale bytes per fragment row of a pair, [pair slot][fragment]
+  [[maybe_unused]] uint32_t xsc[kMx ? 2 : 1][FM], wsc[kMx ? 2 : 1][FN];
+  auto read_scale = [&](int slot, int f) {  // weights first
+    const uint8_t *sc = smem + L::kScale0 + slot * kScaleSlot + (lane >> 5) * 4;
+    if (f < FN) wsc[slot][f] = *reinterpret_cast<const uint32_t *>(sc + 256 * 8 + (row_w + f * 32) * 8);
+    else xsc[slot][f - FN] = *reinterpret_cast<const uint32_t *>(sc + (row_x + (f - FN) * 32) * 8);
+  };
+
   // defined by each tile's first sub-stage (mma0), read by its epilogue
   typename T::acc_t acc[FN][FM];
 
@@ -234,16 +272,16 @@ void gemm_w4_kernel(GemmArgs p) {
   auto epilogue = [&](auto on_block) {
     int m0, n0;
     tile_origin<256, 256>(t_first + tile_i * wgs_per_xcd, p.tiles_m, p.tiles_n, p.group_m, m0, n0);
-    const uint8_t *prm = smem + kParamBase + (tile_i % kParamSets) * kParamBytes;
+    const uint8_t *prm = smem + kParamBase + (tile_i % kParamSets) * L::kParam;
     const float *psa = reinterpret_cast<const float *>(prm);
     const float *psw = reinterpret_cast<const float *>(prm + 1024);
-    const uint8_t *pb = prm + 2048;
+    const uint8_t *pb = prm + L::kBias;
     // the lane index, opaque: the epilogue's addresses are formed here, not
     // hoisted into registers the stage loop needs
     int el = lane;
     asm volatile("" : "+v"(el));
     const int wrow = el & 31, half = el >> 5;
-    uint8_t *xb = smem + kXposeBase + wave * kXpose;
+    uint8_t *xb = smem + L::kXpose0 + wave * kXpose;
     // this lane's write position (row wrow, 8-byte chunk half + constant), and
     // read position (16 bytes: row (el >> 3) + 8 q, chunk el & 7)
     uint8_t *xw = xb + wrow * kXposeRow + half * 8;
@@ -252,7 +290,7 @@ void gemm_w4_kernel(GemmArgs p) {
     // the per-token scales of this lane's rows, one per j (the same in both halves)
     float sam4[FM];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) sam4[j] = p.sa_stride ? psa[wm * kWaveRows + j * 32 + wrow] : sa0;
+    for (int j = 0; j < FM; ++j) sam4[j] = kMx ? 1.0f : p.sa_stride ? psa[wm * kWaveRows + j * 32 + wrow] : sa0;
     // The read-back of step (h, j) is stored during step (h, j) + 1, after that
     // step's writes to the same transpose rows: the reads were issued first, and
     // a wave's LDS operations complete in order, so they return step (h, j)'s
@@ -301,7 +339,7 @@ void gemm_w4_kernel(GemmArgs p) {
       // so they issue together and are waited for once)
       f32x4 swr[2][4], bir[2][4];
       const int nl0 = wn * kWaveRows + 2 * h * 32 + half * 4;  // + ii*32 + gq*8
-      if (p.sw_stride) {
+      if (!kMx && p.sw_stride) {
 #pragma unroll
         for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
@@ -369,7 +407,8 @@ void gemm_w4_kernel(GemmArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float a = T::to_f32(acc[i][j][gq * 4 + e]);
-              y[e] = __builtin_fmaf(a, sam * swr[ii][gq][e], bir[ii][gq][e]);
+              if constexpr (kMx) y[e] = a + bir[ii][gq][e];
+              else y[e] = __builtin_fmaf(a, sam * swr[ii][gq][e], bir[ii][gq][e]);
               if constexpr (ACT == XGEN_ACT_GELU_TANH) y[e] = gelu_tanh(round_out<OUT_DT>(y[e]));
             }
             // row wrow, 8-byte chunk ii*8 + gq*2 + half
@@ -474,9 +513,19 @@ void gemm_w4_kernel(GemmArgs p) {
         if (i == 0) xw = MfmaA<KIND>::widen_x(xf[cb][ks][j]);
         if (fresh && ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[cb][ks][i], xw);
         else MfmaA<KIND>::mma(acc[i][j], wf[cb][ks][i], xw);
+      } else if constexpr (kMx) {
+        // (s is a constant once unrolled: one of the branches stays)
+        const uint32_t sw = wsc[u >> 1][i], sx = xsc[u >> 1][j];
+        if (fresh && ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[cb][ks][i], xf[cb][ks][j], sw, sx);
+        else if (ks == 0) MfmaA<KIND>::template mma<cb * 2>(acc[i][j], wf[cb][ks][i], xf[cb][ks][j], sw, sx);
+        else MfmaA<KIND>::template mma<cb * 2 + 1>(acc[i][j], wf[cb][ks][i], xf[cb][ks][j], sw, sx);
       } else {
         if (fresh && ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[cb][ks][i], xf[cb][ks][j]);
         else MfmaA<KIND>::mma(acc[i][j], wf[cb][ks][i], xf[cb][ks][j]);
+      }
+      if constexpr (kMx && read && odd) {  // the next pair's scales, with its first fragments
+#pragma unroll
+        for (int f = spread_first(s, FM + FN, kMfmas); f < spread_first(s + 1, FM + FN, kMfmas); ++f) read_scale(ns >> 1, f);
       }
       if constexpr (read) {
 #pragma unroll
@@ -496,6 +545,10 @@ void gemm_w4_kernel(GemmArgs p) {
   };
   // stage 0's fragments (slot 0, register buffer 0)
   auto read_first = [&]() {
+    if constexpr (kMx) {
+#pragma unroll
+      for (int f = 0; f < FM + FN; ++f) read_scale(0, f);
+    }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -513,8 +566,13 @@ void gemm_w4_kernel(GemmArgs p) {
     epilogue([&](int i, int j, int b) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if (ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
-        else MfmaA<KIND>::mma(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
+        if constexpr (kMx) {
+          if (ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[0][ks][i], xf[0][ks][j], wsc[0][i], xsc[0][j]);
+          else MfmaA<KIND>::template mma<1>(acc[i][j], wf[0][ks][i], xf[0][ks][j], wsc[0][i], xsc[0][j]);
+        } else {
+          if (ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
+          else MfmaA<KIND>::mma(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
+        }
       }
       (void)b;
     });
@@ -546,7 +604,7 @@ void gemm_w4_kernel(GemmArgs p) {
 #pragma unroll
     for (int q = 0; q < kLoadsPerPair; ++q) issue_load(is, 1, q);
     issue_end();
-    wait_vmcnt<kLoadsPerPair>();
+    wait_vmcnt<kLoadsPerPair + (kMx ? 1 : 0)>();
     lds_barrier();
     read_first();
   }
@@ -590,6 +648,11 @@ void launch_gemm_w4(const GemmArgs &a, bool acc_out, hipStream_t stream) {
   else gemm_w4_kernel<KIND, ACT, OUT_DT, false, false><<<grid, block, 0, stream>>>(a);
 }
 
+template <int KIND, int ACT, int OUT_DT>
+void launch_gemm_plain(const GemmArgs &a, hipStream_t stream) {
+  gemm_w4_kernel<KIND, ACT, OUT_DT, false, false><<<gemm_grid(a), dim3(w4::kThreads), 0, stream>>>(a);
+}
+
 template <int KIND>
 void launch_gemm_w4_gated(const GemmArgs &a, hipStream_t stream) {
   gemm_w4_kernel<KIND, XGEN_ACT_NONE, XGEN_DTYPE_BF16, false, true>
@@ -605,12 +668,21 @@ struct GateParams {  // the gated residual epilogue's inputs (null residual: pla
   int64_t seq = 0;
 };
 
+struct BlockScales {  // the MXFP4 kind's scale bytes (xgen_mxfp4_quantize's layout) in place of sa and sw
+  const uint8_t *x = nullptr;
+  int64_t x_block = 0;  // bytes between the blocks of 256 values
+  const uint8_t *w = nullptr;
+  int64_t w_block = 0;
+};
+
+// (KIND kMx4: K, lda and ldw in bytes)
 template <int KIND>
 int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_t ldw, int64_t M,
                int64_t N, int64_t K, const float *sa, int64_t sa_stride, const float *sw,
                int64_t sw_stride, const void *bias, int bias_dtype, int activation, void *out,
                int out_dtype, int64_t ldo, void *acc_out, hipStream_t stream,
-               const GateParams &gp = GateParams()) {
+               const GateParams &gp = GateParams(), const BlockScales &bs = BlockScales()) {
+  constexpr bool kMx = KIND == kMx4;
   const bool gated = gp.residual != nullptr;
   if (M < 0 || N <= 0 || K <= 0)
     return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: bad shape M=%lld N=%lld K=%lld", fn, (long long)M,
@@ -626,7 +698,8 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   if (out_dtype != XGEN_DTYPE_BF16 && out_dtype != XGEN_DTYPE_F16)
     return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: output dtype must be BF16 or F16", fn);
   if (M == 0) return ok();
-  if (!a || !w || !sa || !sw || !out) return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (!a || !w || (kMx ? !bs.x || !bs.w : !sa || !sw) || !out)
+    return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
   if (K % 16 || N % 16) return fail(XGEN_ERR_UNSUPPORTED, "%s: K and N must be multiples of 16", fn);
   if (lda % 16 || ldw % 16 || !aligned16(a) || !aligned16(w))
     return fail(XGEN_ERR_UNSUPPORTED, "%s: operand rows must be 16-byte aligned", fn);
@@ -665,10 +738,12 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
       const int64_t mi = M - m0 < rows ? M - m0 : rows;
       GateParams gc = gp;
       if (gated) gc.residual = static_cast<const uint8_t *>(gp.residual) + m0 * gp.ld_residual * 2;
+      BlockScales bc = bs;
+      if (kMx) bc.x = bs.x + m0 * 8;
       const int st = gemm_entry<KIND>(
           fn, static_cast<const uint8_t *>(a) + m0 * lda, lda, w, ldw, mi, N, K, sa_stride ? sa + m0 : sa, sa_stride,
           sw, sw_stride, bias, bias_dtype, activation, static_cast<uint8_t *>(out) + m0 * ldo * 2, out_dtype, ldo,
-          acc_out ? static_cast<uint8_t *>(acc_out) + m0 * N * 4 : nullptr, stream, gc);
+          acc_out ? static_cast<uint8_t *>(acc_out) + m0 * N * 4 : nullptr, stream, gc, bc);
       if (st != XGEN_OK) return st;
     }
     return ok();
@@ -725,6 +800,12 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   }
   g.residual_bytes = gated ? (uint32_t)(((M - 1) * gp.ld_residual + N) * 2) : 0;
   g.gate_bytes = gated ? (uint32_t)(((gp.gate_rows - 1) * gp.gate_stride + N) * 2) : 0;
+  g.xs = bs.x;
+  g.ws = bs.w;
+  g.xs_block = bs.x_block;
+  g.ws_block = bs.w_block;
+  g.xs_rows = (uint32_t)((M + M % 2) * 8);  // (below 2^31: M rows of at least 16 bytes are)
+  g.ws_rows = (uint32_t)(N * 8);
   g.kt4 = (int)(((K + BK - 1) / BK + 3) / 4 * 4);
   const int64_t out_bytes = ((M - 1) * ldo + N) * 2;
   if (out_bytes >= (int64_t)kOutOfRange)
@@ -741,7 +822,13 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
     return launch_status(fn);
   }
   const bool with_acc = acc_out != nullptr;
-  if (gated) {
+  if constexpr (kMx) {
+    if (gated) launch_gemm_w4_gated<KIND>(g, stream);
+    else if (activation == XGEN_ACT_NONE && out_dtype == XGEN_DTYPE_BF16) launch_gemm_plain<KIND, XGEN_ACT_NONE, XGEN_DTYPE_BF16>(g, stream);
+    else if (activation == XGEN_ACT_NONE) launch_gemm_plain<KIND, XGEN_ACT_NONE, XGEN_DTYPE_F16>(g, stream);
+    else if (out_dtype == XGEN_DTYPE_BF16) launch_gemm_plain<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_BF16>(g, stream);
+    else launch_gemm_plain<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_F16>(g, stream);
+  } else if (gated) {
     // (the gated entry takes the FP8 and INT8 kinds only: no exact-kind instance)
     if constexpr (KIND != kFp8Exact) launch_gemm_w4_gated<KIND>(g, stream);
   } else if (activation == XGEN_ACT_NONE) {
@@ -815,4 +902,38 @@ extern "C" int xgen_w8a8_gate_residual(int in_dtype, const void *a, int64_t lda,
                             bias_dtype, XGEN_ACT_NONE, out, XGEN_DTYPE_BF16, ldo, nullptr, stream, gp);
   return gemm_entry<kInt8>(fn, a, lda, w, ldw, M, N, K, a_scale, a_scale_stride, w_scale, w_scale_stride, bias,
                            bias_dtype, XGEN_ACT_NONE, out, XGEN_DTYPE_BF16, ldo, nullptr, stream, gp);
+}
+
+extern "C" int xgen_mxfp4_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_block_stride,
+                                 const void *w, int64_t ldw, const void *w_scales, int64_t w_block_stride, int64_t M,
+                                 int64_t N, int64_t K, const void *bias, int bias_dtype, int activation,
+                                 const void *residual, int64_t ld_residual, const void *gate_table,
+                                 int64_t gate_row_stride, int64_t gate_rows, const int64_t *indices, int64_t seq,
+                                 void *out, int out_dtype, int64_t ldo, hipStream_t stream) {
+  const char *fn = "xgen_mxfp4_matmul";
+  if (M < 0 || N <= 0 || K <= 0)
+    return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: bad shape M=%lld N=%lld K=%lld", fn, (long long)M, (long long)N,
+                (long long)K);
+  if (K % 32) return fail(XGEN_ERR_UNSUPPORTED, "%s: K must be a multiple of 32", fn);
+  if (a_block_stride < (M + M % 2) * 8 || w_block_stride < (N + N % 2) * 8)
+    return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: the scales' blocks must cover the rows", fn);
+  if (a_block_stride % 16 || w_block_stride % 16 || !aligned16(a_scales) || !aligned16(w_scales))
+    return fail(XGEN_ERR_UNSUPPORTED, "%s: the scales' blocks must be 16-byte aligned", fn);
+  if (residual && (activation != XGEN_ACT_NONE || out_dtype != XGEN_DTYPE_BF16))
+    return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: a gated residual takes no activation and a BF16 output", fn);
+  GateParams gp;
+  gp.residual = residual;
+  gp.ld_residual = ld_residual;
+  gp.gate = gate_table;
+  gp.gate_stride = gate_row_stride;
+  gp.gate_rows = gate_rows;
+  gp.indices = indices;
+  gp.seq = seq;
+  BlockScales bs;
+  bs.x = static_cast<const uint8_t *>(a_scales);
+  bs.x_block = a_block_stride;
+  bs.w = static_cast<const uint8_t *>(w_scales);
+  bs.w_block = w_block_stride;
+  return gemm_entry<kMx4>(fn, a, lda, w, ldw, M, N, K / 2, nullptr, 0, nullptr, 0, bias, bias_dtype, activation, out,
+                          out_dtype, ldo, nullptr, stream, gp, bs);
 }

@@ -40,7 +40,8 @@ struct Api {
   // added within ABI version 1: null where XGEN_AMD_LIBRARY names a library from before them
 #define XGEN_ADDED(X)                                                                                       \
   X(xgen_fp8_quantize_tensor) X(xgen_residual_norm) X(xgen_route_workspace_bytes) X(xgen_route)             \
-  X(xgen_grouped_matmul) X(xgen_expert_combine)
+  X(xgen_grouped_matmul) X(xgen_expert_combine) X(xgen_mxfp4_quantize) X(xgen_mxfp4_dequantize)            \
+  X(xgen_mxfp4_matmul) X(xgen_qk_norm_rope) X(xgen_rotary_table)
   XGEN_ADDED(XGEN_FIELD)
 };
 
@@ -620,6 +621,194 @@ Tensor expert_combine(const Tensor &y_in, const Tensor &weights_in, const Tensor
   return out;
 }
 
+// --- 4-bit rows and their product --------------------------------------------------------------
+at::DimVector mx_scales_shape(int64_t rows, int64_t K) { return {(K + 255) / 256, rows + rows % 2, 8}; }
+
+std::tuple<Tensor, Tensor> quantize_mxfp4(const Tensor &x, int64_t rounding) {
+  on_gpu(x);
+  TORCH_CHECK(is_half(x), "quantize_mxfp4: BF16/F16 input required");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 32 == 0,
+              "quantize_mxfp4: a last dimension in multiples of 32 required");
+  TORCH_CHECK(rounding == XGEN_MX_FLOOR || rounding == XGEN_MX_CEIL, "quantize_mxfp4: rounding must be 0 (floor) or 1 (ceil)");
+  const auto entry = added(api().xgen_mxfp4_quantize, "xgen_mxfp4_quantize");
+  const c10::DeviceGuard guard(x.device());
+  const int64_t K = x.size(-1), rows = x.numel() / K;
+  at::DimVector shape(x.sizes());
+  shape.back() = K / 2;
+  Tensor codes = empty(shape, at::kByte, x), scales = empty(mx_scales_shape(rows, K), at::kByte, x);
+  if (rows == 0) return {codes, scales};
+  Tensor m = rows_view(x);
+  if (!aligned16(m) || rows_apart(m) % 8) m = m.clone(at::MemoryFormat::Contiguous);
+  check(entry(dtype_code(x.scalar_type()), m.data_ptr(), rows, K, rows_apart(m), (int)rounding, codes.data_ptr(), K / 2,
+              scales.data_ptr(), scales.stride(0), stream_of(x)),
+        "xgen_mxfp4_quantize");
+  return {codes, scales};
+}
+
+// Packed rows as the kernels read them: codes [rows, K / 2] with aligned rows, scales contiguous and aligned.
+struct MxRows {
+  Tensor codes, scales;
+  int64_t rows, K, ld, block;
+  MxRows(const char *what, const Tensor &codes_in, const Tensor &scales_in, const char *name) {
+    TORCH_CHECK(codes_in.scalar_type() == at::kByte && codes_in.dim() >= 1 && codes_in.size(-1) > 0 && codes_in.size(-1) % 16 == 0,
+                what, ": ", name, " uint8 [..., K/2] with K a multiple of 32 required");
+    K = codes_in.size(-1) * 2;
+    rows = codes_in.numel() / codes_in.size(-1);
+    TORCH_CHECK(scales_in.scalar_type() == at::kByte && scales_in.sizes() == at::IntArrayRef(mx_scales_shape(rows, K)),
+                what, ": ", name, " scales uint8 [ceil(K/256), rows rounded up to even, 8] required");
+    codes = codes_in;
+    scales = scales_in;
+  }
+  void lay_out() {
+    if (rows == 0) return;
+    codes = rows_view(codes);
+    if (!aligned16(codes) || rows_apart(codes) % 16) codes = codes.clone(at::MemoryFormat::Contiguous);
+    ld = rows_apart(codes);
+    scales = aligned_flat(scales);
+    block = (rows + rows % 2) * 8;
+  }
+};
+
+Tensor dequantize_mxfp4(const Tensor &codes_in, const Tensor &scales_in, at::ScalarType out_dtype) {
+  const char *what = "dequantize_mxfp4";
+  on_gpu(codes_in, scales_in);
+  MxRows m(what, codes_in, scales_in, "codes");
+  TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kHalf || out_dtype == at::kFloat,
+              what, ": out_dtype must be bfloat16, float16 or float32");
+  const auto entry = added(api().xgen_mxfp4_dequantize, "xgen_mxfp4_dequantize");
+  const c10::DeviceGuard guard(codes_in.device());
+  at::DimVector shape(codes_in.sizes());
+  shape.back() = m.K;
+  Tensor out = empty(shape, out_dtype, codes_in);
+  if (m.rows == 0) return out;
+  m.lay_out();
+  check(entry(m.codes.data_ptr(), m.ld, m.scales.data_ptr(), m.block, m.rows, m.K, dtype_code(out_dtype), out.data_ptr(),
+              m.K, stream_of(codes_in)),
+        "xgen_mxfp4_dequantize");
+  return out;
+}
+
+Tensor mxfp4_matmul(const Tensor &a_in, const Tensor &a_scales, const Tensor &w_in, const Tensor &w_scales,
+                    const OptTensor &bias_in, at::ScalarType out_dtype, int64_t activation, const OptTensor &residual_in,
+                    const OptTensor &gate_in, const OptTensor &indices_in) {
+  const char *what = "mxfp4_matmul";
+  on_gpu(a_in, a_scales, w_in, w_scales, bias_in, residual_in, gate_in, indices_in);
+  TORCH_CHECK(a_in.dim() == 2 && w_in.dim() == 2 && a_in.size(1) == w_in.size(1), what, ": a [M,K/2] and w [N,K/2] required");
+  MxRows a(what, a_in, a_scales, "a"), w(what, w_in, w_scales, "w");
+  const int64_t M = a.rows, Nf = w.rows;
+  TORCH_CHECK(Nf > 0 && Nf % 16 == 0, what, ": N must be a positive multiple of 16");
+  TORCH_CHECK(!bias_in || (bias_in->dim() == 1 && bias_in->size(0) == Nf && (is_half(*bias_in) || bias_in->scalar_type() == at::kFloat)),
+              what, ": bias [N] of BF16/F16/F32 required");
+  TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kHalf, what, ": out_dtype must be bfloat16 or float16");
+  TORCH_CHECK(activation == XGEN_ACT_NONE || activation == XGEN_ACT_GELU_TANH, what, ": activation must be 0 (none) or 1 (gelu_tanh)");
+  const bool gated = residual_in.has_value();
+  TORCH_CHECK(gated == gate_in.has_value() && gated == indices_in.has_value(), what, ": residual, gate_table and indices come together");
+  if (gated) {
+    TORCH_CHECK(activation == XGEN_ACT_NONE && out_dtype == at::kBFloat16,
+                what, ": a gated residual takes no activation and a bfloat16 output");
+    TORCH_CHECK(residual_in->sizes() == at::IntArrayRef({M, Nf}) && residual_in->scalar_type() == at::kBFloat16,
+                what, ": residual BF16 [M, N] required");
+    TORCH_CHECK(gate_in->dim() == 2 && gate_in->size(1) == Nf && gate_in->size(0) > 0 && gate_in->scalar_type() == at::kBFloat16,
+                what, ": gate_table BF16 [T, N] required");
+    TORCH_CHECK(indices_in->dim() == 1 && indices_in->scalar_type() == at::kLong && indices_in->size(0) > 0 && M % indices_in->size(0) == 0,
+                what, ": int64 indices [S] with M % S == 0 required");
+  }
+  const auto entry = added(api().xgen_mxfp4_matmul, "xgen_mxfp4_matmul");
+  const c10::DeviceGuard guard(a_in.device());
+  Tensor out = empty({M, Nf}, out_dtype, a_in);
+  if (M == 0) return out;
+  a.lay_out();
+  w.lay_out();
+  const Tensor bias = optional_flat(bias_in), residual = gated ? kernel_rows(*residual_in, 8) : Tensor();
+  const Tensor gate = gated ? kernel_rows(*gate_in, 8) : Tensor(), indices = gated ? indices_in->contiguous() : Tensor();
+  check(entry(a.codes.data_ptr(), a.ld, a.scales.data_ptr(), a.block, w.codes.data_ptr(), w.ld, w.scales.data_ptr(), w.block,
+              M, Nf, a.K, optional_ptr(bias), bias.defined() ? dtype_code(bias.scalar_type()) : XGEN_DTYPE_NONE, (int)activation,
+              optional_ptr(residual), gated ? residual.stride(0) : 0, optional_ptr(gate), gated ? gate.stride(0) : 0,
+              gated ? gate.size(0) : 0, gated ? indices.data_ptr<int64_t>() : nullptr, gated ? indices.size(0) : 0,
+              out.data_ptr(), dtype_code(out_dtype), out.stride(0), stream_of(a_in)),
+        "xgen_mxfp4_matmul");
+  return out;
+}
+
+// --- queries and keys ----------------------------------------------------------------------------
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor &q_in, const Tensor &k_in, const Tensor &cos_in, const Tensor &sin_in,
+                                        const OptTensor &positions_in, const OptTensor &q_weight, const OptTensor &k_weight,
+                                        int64_t norm_kind, double eps, bool interleaved) {
+  const char *what = "qk_norm_rope";
+  on_gpu(q_in, k_in, cos_in, sin_in, positions_in, q_weight, k_weight);
+  TORCH_CHECK(q_in.dim() == 4 && k_in.dim() == 4 && is_half(q_in) && k_in.scalar_type() == q_in.scalar_type() &&
+                  q_in.size(0) == k_in.size(0) && q_in.size(1) == k_in.size(1) && q_in.size(3) == k_in.size(3),
+              what, ": q [B,S,H,D] and k [B,S,Hk,D] of one dtype, BF16 or F16, required");
+  const int64_t B = q_in.size(0), S = q_in.size(1), D = q_in.size(3);
+  TORCH_CHECK(D > 0 && D <= XGEN_HEAD_MAX_DIM && D % 8 == 0, what, ": D a multiple of 8, up to ", XGEN_HEAD_MAX_DIM, ", required");
+  TORCH_CHECK(cos_in.dim() == 2 && sin_in.sizes() == cos_in.sizes() && cos_in.scalar_type() == at::kFloat &&
+                  sin_in.scalar_type() == at::kFloat && cos_in.size(1) > 0 && cos_in.size(1) <= D / 2,
+              what, ": float32 cos and sin [P,R/2] with 0 < R <= D required");
+  TORCH_CHECK(!positions_in || (positions_in->scalar_type() == at::kLong &&
+                                (positions_in->sizes() == at::IntArrayRef({S}) || positions_in->sizes() == at::IntArrayRef({B, S}))),
+              what, ": int64 positions [S] or [B,S] or None required");
+  TORCH_CHECK(norm_kind == XGEN_NORM_NONE || norm_kind == XGEN_NORM_LAYER || norm_kind == XGEN_NORM_RMS,
+              what, ": norm_kind must be -1 (none), 0 (layer) or 1 (rms)");
+  for (const OptTensor *w : {&q_weight, &k_weight}) {
+    TORCH_CHECK(!*w || ((*w)->dim() == 1 && (*w)->size(0) == D && (is_half(**w) || (*w)->scalar_type() == at::kFloat)),
+                what, ": BF16/F16/F32 weights [D] or None required");
+    TORCH_CHECK(!*w || norm_kind != XGEN_NORM_NONE, what, ": a weight needs a norm");
+  }
+  TORCH_CHECK((float)eps >= std::numeric_limits<float>::min() && (float)eps < 1.0f, what, ": eps must be in [2^-126, 1) as a float32");
+  const auto entry = added(api().xgen_qk_norm_rope, "xgen_qk_norm_rope");
+  const c10::DeviceGuard guard(q_in.device());
+  Tensor q_out = empty(q_in.sizes(), q_in.scalar_type(), q_in), k_out = empty(k_in.sizes(), q_in.scalar_type(), q_in);
+  if (q_out.numel() + k_out.numel() == 0) return {q_out, k_out};
+  auto heads = [](const Tensor &t) {
+    bool ok = t.stride(3) == 1 && aligned16(t);
+    for (int64_t d = 0; d < 3; ++d) ok = ok && t.stride(d) % 8 == 0;
+    return ok || t.numel() == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+  };
+  const Tensor q = heads(q_in), k = heads(k_in), cos = cos_in.contiguous(), sin = sin_in.contiguous();
+  Tensor wq = q_weight ? q_weight->contiguous() : Tensor(), wk = k_weight ? k_weight->contiguous() : Tensor();
+  if (wq.defined() && wk.defined() && wq.scalar_type() != wk.scalar_type()) {  // one dtype for both: the wider, exactly
+    wq = wq.to(at::kFloat);
+    wk = wk.to(at::kFloat);
+  }
+  const Tensor positions = positions_in ? positions_in->contiguous() : Tensor();
+  check(entry(dtype_code(q.scalar_type()), q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), q.size(2), k.data_ptr(),
+              k.stride(0), k.stride(1), k.stride(2), k.size(2), B, S, D, (int)norm_kind, optional_ptr(wq), optional_ptr(wk),
+              wq.defined()   ? dtype_code(wq.scalar_type())
+              : wk.defined() ? dtype_code(wk.scalar_type())
+                             : XGEN_DTYPE_NONE,
+              (float)eps, cos.data_ptr<float>(), sin.data_ptr<float>(), cos.size(0), cos.size(1), interleaved ? 1 : 0,
+              positions.defined() ? positions.data_ptr<int64_t>() : nullptr,
+              positions.defined() && positions.dim() == 2 ? S : 0, q_out.data_ptr(), k_out.data_ptr(), stream_of(q_in)),
+        "xgen_qk_norm_rope");
+  return {q_out, k_out};
+}
+
+std::tuple<Tensor, Tensor> rotary_table(const Tensor &positions_in, const Tensor &frequencies_in, const OptTensor &axes_in,
+                                        double factor) {
+  const char *what = "rotary_table";
+  on_gpu(positions_in, frequencies_in, axes_in);
+  TORCH_CHECK(positions_in.scalar_type() == at::kLong && (positions_in.dim() == 1 || positions_in.dim() == 2),
+              what, ": int64 positions [P] or [P,A] required");
+  const int64_t P = positions_in.size(0), A = positions_in.dim() == 2 ? positions_in.size(1) : 1;
+  TORCH_CHECK(A > 0, what, ": one axis at least");
+  TORCH_CHECK(frequencies_in.dim() == 1 && frequencies_in.scalar_type() == at::kDouble, what, ": float64 frequencies [R/2] required");
+  const int64_t R = frequencies_in.size(0);
+  TORCH_CHECK(!axes_in || (axes_in->sizes() == frequencies_in.sizes() && axes_in->scalar_type() == at::kInt),
+              what, ": int32 axes [R/2] or None required");
+  TORCH_CHECK(std::isfinite(factor), what, ": factor must be finite");
+  TORCH_CHECK(R == 0 || P <= 0x7fffffffLL / R, what, ": P*R/2 must be below 2^31");
+  const auto entry = added(api().xgen_rotary_table, "xgen_rotary_table");
+  const c10::DeviceGuard guard(positions_in.device());
+  Tensor cos = empty({P, R}, at::kFloat, positions_in), sin = empty({P, R}, at::kFloat, positions_in);
+  if (cos.numel() == 0) return {cos, sin};
+  const Tensor positions = positions_in.contiguous(), frequencies = frequencies_in.contiguous();
+  const Tensor axes = axes_in ? axes_in->contiguous() : Tensor();
+  check(entry(positions.data_ptr<int64_t>(), P, A, frequencies.data_ptr<double>(), axes.defined() ? axes.data_ptr<int>() : nullptr,
+              R, factor, cos.data_ptr<float>(), sin.data_ptr<float>(), stream_of(positions_in)),
+        "xgen_rotary_table");
+  return {cos, sin};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(xgen_amd, CUDA, m) {
@@ -638,4 +827,9 @@ TORCH_LIBRARY_IMPL(xgen_amd, CUDA, m) {
   m.impl("route", route);
   m.impl("grouped_matmul", grouped_matmul);
   m.impl("expert_combine", expert_combine);
+  m.impl("quantize_mxfp4", quantize_mxfp4);
+  m.impl("dequantize_mxfp4", dequantize_mxfp4);
+  m.impl("mxfp4_matmul", mxfp4_matmul);
+  m.impl("qk_norm_rope", qk_norm_rope);
+  m.impl("rotary_table", rotary_table);
 }

@@ -30,6 +30,7 @@ from torch import nn
 from .. import _native as N
 from ..config import QuantLayerConfig, detect_config_name, get_config
 from ..ops import xops
+from .mxfp4 import MXFP4Linear
 
 LOG = logging.getLogger(__name__)
 
@@ -113,15 +114,16 @@ def quant_matmul_raw(q, scale, linear, out_dtype=torch.bfloat16, activation=N.AC
 
 
 def enable_weight_quant_linear(model: nn.Module, quant_config: QuantLayerConfig, dtype: str = 'w8a8') -> nn.Module:
-    """Replace every selected nn.Linear by a WeightQuantLinearModule (matmul.py:141-202).
+    """Replace every selected nn.Linear by a WeightQuantLinearModule (matmul.py:141-202), or an MXFP4Linear.
 
     Selection is quant_config.should_quantize(name, layer); layers whose weight
     was released are skipped; LoRA '.base_layer' suffixes are undone in the
-    replacement name.  Only W8A8 is provided (the reference's transformer path
-    builds the W8A8 module for every CLI value, matmul.py:183).
+    replacement name.  dtype 'w8a8' (the reference's transformer path builds the
+    W8A8 module for every CLI value, matmul.py:183) or 'mxfp4': MXFP4Linear modules,
+    4-bit weights and activations.
     """
-    if dtype != 'w8a8':
-        raise ValueError("xgen_amd provides the W8A8 module only")
+    if dtype not in ('w8a8', 'mxfp4'):
+        raise ValueError("xgen_amd provides 'w8a8' and 'mxfp4' modules")
     for name, layer in list(model.named_modules()):
         if not quant_config.should_quantize(name, layer):
             continue
@@ -129,7 +131,11 @@ def enable_weight_quant_linear(model: nn.Module, quant_config: QuantLayerConfig,
             continue
         clean_name = name.replace(".base_layer", "")
         bias = layer.bias.data if getattr(layer, 'bias', None) is not None else None
-        quant_module = WeightQuantLinearModule(layer.weight.data, bias, clean_name)
+        if dtype == 'mxfp4':
+            weight = layer.weight.data
+            quant_module = MXFP4Linear(weight.to(torch.bfloat16) if weight.dtype == torch.float32 else weight, bias)
+        else:
+            quant_module = WeightQuantLinearModule(layer.weight.data, bias, clean_name)
         if '.' in clean_name:
             parent, leaf = clean_name.rsplit('.', 1)
             setattr(model.get_submodule(parent), leaf, quant_module)

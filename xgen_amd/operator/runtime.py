@@ -210,6 +210,8 @@ class Kernels:
         "merge_quant": ("merge_quant", None),
         "residual_norm": ("residual_norm", None),
         "experts": ("experts", None),
+        "mxfp4": ("mxfp4", None),
+        "qk_norm_rope": ("qk_norm_rope", None),
     }
 
     def __init__(self, diagnostics):

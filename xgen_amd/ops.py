@@ -59,6 +59,16 @@ SCHEMAS = {
     "expert_combine": (
         "expert_combine(Tensor y, Tensor weights, Tensor slots, Tensor? residual, Tensor? gate_table, "
         "Tensor? indices) -> Tensor"),
+    "quantize_mxfp4": "quantize_mxfp4(Tensor x, int rounding) -> (Tensor, Tensor)",
+    "dequantize_mxfp4": "dequantize_mxfp4(Tensor codes, Tensor scales, ScalarType out_dtype) -> Tensor",
+    "mxfp4_matmul": (
+        "mxfp4_matmul(Tensor a, Tensor a_scales, Tensor w, Tensor w_scales, Tensor? bias, ScalarType out_dtype, "
+        "int activation, Tensor? residual, Tensor? gate_table, Tensor? indices) -> Tensor"),
+    "qk_norm_rope": (
+        "qk_norm_rope(Tensor q, Tensor k, Tensor cos, Tensor sin, Tensor? positions, Tensor? q_weight, "
+        "Tensor? k_weight, int norm_kind, float eps, bool interleaved) -> (Tensor, Tensor)"),
+    "rotary_table": (
+        "rotary_table(Tensor positions, Tensor frequencies, Tensor? axes, float factor) -> (Tensor, Tensor)"),
 }
 
 
@@ -331,6 +341,94 @@ def _combine_meta(y, weights, slots, residual, gate_table, indices):
     return torch.empty((T, H), dtype=y.dtype, device=y.device)
 
 
+def _mx_scales_shape(rows, K):
+    return ((K + 255) // 256, rows + rows % 2, 8)
+
+
+def _mx_quantize_meta(x, rounding):
+    what = "quantize_mxfp4"
+    _require(x.dtype in (torch.bfloat16, torch.float16), f"{what}: BF16/F16 input required")
+    _require(x.dim() >= 1 and x.shape[-1] > 0 and x.shape[-1] % 32 == 0, f"{what}: a last dimension in multiples of 32 required")
+    _require(rounding in (N.MX_FLOOR, N.MX_CEIL), f"{what}: rounding must be 0 (floor) or 1 (ceil)")
+    K = x.shape[-1]
+    return (torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=x.device),
+            torch.empty(_mx_scales_shape(x.numel() // K, K), dtype=torch.uint8, device=x.device))
+
+
+def _mx_rows(what, codes, scales, name):
+    """(rows, K) of checked packed rows."""
+    _require(codes.dtype == torch.uint8 and codes.dim() >= 1 and codes.shape[-1] > 0 and codes.shape[-1] % 16 == 0,
+             f"{what}: {name} uint8 [..., K/2] with K a multiple of 32 required")
+    K = codes.shape[-1] * 2
+    rows = codes.numel() // codes.shape[-1]
+    _require(scales.dtype == torch.uint8 and tuple(scales.shape) == _mx_scales_shape(rows, K),
+             f"{what}: {name} scales uint8 [ceil(K/256), rows rounded up to even, 8] required")
+    return rows, K
+
+
+def _mx_dequantize_meta(codes, scales, out_dtype):
+    what = "dequantize_mxfp4"
+    _, K = _mx_rows(what, codes, scales, "codes")
+    _require(out_dtype in (torch.bfloat16, torch.float16, torch.float32), f"{what}: out_dtype must be bfloat16, float16 or float32")
+    return torch.empty((*codes.shape[:-1], K), dtype=out_dtype, device=codes.device)
+
+
+def _mx_matmul_meta(a, a_scales, w, w_scales, bias, out_dtype, activation, residual, gate_table, indices):
+    what = "mxfp4_matmul"
+    _require(a.dim() == 2 and w.dim() == 2 and a.shape[1] == w.shape[1], f"{what}: a [M,K/2] and w [N,K/2] required")
+    M, _ = _mx_rows(what, a, a_scales, "a")
+    Nf, _ = _mx_rows(what, w, w_scales, "w")
+    _require(Nf > 0 and Nf % 16 == 0, f"{what}: N must be a positive multiple of 16")
+    _require(bias is None or (bias.dim() == 1 and bias.shape[0] == Nf
+                              and bias.dtype in (torch.bfloat16, torch.float16, torch.float32)),
+             f"{what}: bias [N] of BF16/F16/F32 required")
+    _require(out_dtype in (torch.bfloat16, torch.float16), f"{what}: out_dtype must be bfloat16 or float16")
+    _require(activation in (N.ACT_NONE, N.ACT_GELU_TANH), f"{what}: activation must be 0 (none) or 1 (gelu_tanh)")
+    _require((residual is None) == (gate_table is None) == (indices is None), f"{what}: residual, gate_table and indices come together")
+    if residual is not None:
+        _require(activation == N.ACT_NONE and out_dtype == torch.bfloat16,
+                 f"{what}: a gated residual takes no activation and a bfloat16 output")
+        _require(tuple(residual.shape) == (M, Nf) and residual.dtype == torch.bfloat16, f"{what}: residual BF16 [M, N] required")
+        _require(gate_table.dim() == 2 and gate_table.shape[1] == Nf and gate_table.shape[0] > 0
+                 and gate_table.dtype == torch.bfloat16, f"{what}: gate_table BF16 [T, N] required")
+        _require(indices.dim() == 1 and indices.dtype == torch.int64 and indices.shape[0] > 0 and M % indices.shape[0] == 0,
+                 f"{what}: int64 indices [S] with M % S == 0 required")
+    return torch.empty((M, Nf), dtype=out_dtype, device=a.device)
+
+
+def _qk_meta(q, k, cos, sin, positions, q_weight, k_weight, norm_kind, eps, interleaved):
+    what = "qk_norm_rope"
+    _require(q.dim() == 4 and k.dim() == 4 and q.dtype == k.dtype and q.dtype in (torch.bfloat16, torch.float16)
+             and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3],
+             f"{what}: q [B,S,H,D] and k [B,S,Hk,D] of one dtype, BF16 or F16, required")
+    B, S, _, D = q.shape
+    _require(0 < D <= N.HEAD_MAX_DIM and D % 8 == 0, f"{what}: D a multiple of 8, up to {N.HEAD_MAX_DIM}, required")
+    _require(cos.dim() == 2 and sin.shape == cos.shape and cos.dtype == sin.dtype == torch.float32
+             and 0 < cos.shape[1] <= D // 2, f"{what}: float32 cos and sin [P,R/2] with 0 < R <= D required")
+    _require(positions is None or (positions.dtype == torch.int64 and tuple(positions.shape) in ((S,), (B, S))),
+             f"{what}: int64 positions [S] or [B,S] or None required")
+    _require(norm_kind in (N.NORM_NONE, N.NORM_LAYER, N.NORM_RMS), f"{what}: norm_kind must be -1 (none), 0 (layer) or 1 (rms)")
+    for w in (q_weight, k_weight):
+        _require(w is None or (w.dim() == 1 and w.shape[0] == D and w.dtype in (torch.bfloat16, torch.float16, torch.float32)),
+                 f"{what}: BF16/F16/F32 weights [D] or None required")
+        _require(w is None or norm_kind != N.NORM_NONE, f"{what}: a weight needs a norm")
+    _require(torch.finfo(torch.float32).tiny <= ctypes.c_float(eps).value < 1, f"{what}: eps must be in [2^-126, 1) as a float32")
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+
+
+def _table_meta(positions, frequencies, axes, factor):
+    what = "rotary_table"
+    _require(positions.dtype == torch.int64 and positions.dim() in (1, 2), f"{what}: int64 positions [P] or [P,A] required")
+    _require(positions.dim() == 1 or positions.shape[1] > 0, f"{what}: one axis at least")
+    _require(frequencies.dim() == 1 and frequencies.dtype == torch.float64, f"{what}: float64 frequencies [R/2] required")
+    _require(axes is None or (axes.shape == frequencies.shape and axes.dtype == torch.int32),
+             f"{what}: int32 axes [R/2] or None required")
+    _require(math.isfinite(factor), f"{what}: factor must be finite")
+    P, R = positions.shape[0], frequencies.shape[0]
+    _require(P * R < 2 ** 31, f"{what}: P*R/2 must be below 2^31")
+    return tuple(torch.empty((P, R), dtype=torch.float32, device=positions.device) for _ in range(2))
+
+
 # --------------------------------------------------------------------------- device
 def _on_gpu(*ts):
     dev = ts[0].device
@@ -390,6 +488,11 @@ _META = {
     "route": _route_meta,
     "grouped_matmul": _grouped_meta,
     "expert_combine": _combine_meta,
+    "quantize_mxfp4": _mx_quantize_meta,
+    "dequantize_mxfp4": _mx_dequantize_meta,
+    "mxfp4_matmul": _mx_matmul_meta,
+    "qk_norm_rope": _qk_meta,
+    "rotary_table": _table_meta,
 }
 
 
