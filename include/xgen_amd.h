@@ -593,7 +593,7 @@ int xgen_mxfp4_matmul(const void *a, int64_t lda, const void *a_scales, int64_t 
  * shapes.  norm_kind XGEN_NORM_NONE (no weights), _LAYER or _RMS; weights NULL or [dim] of weight_dtype (BF16/F16/F32).
  * cos, sin: float32 [places, pairs] (xgen_rotary_table's).  p = positions[b * position_stride_batch + s], or s if positions is
  * NULL; a position outside [0, places) makes its token's heads NaN.  dim a multiple of 8, up to XGEN_HEAD_MAX_DIM; strides
- * multiples of 8, heads 16-byte aligned; eps in [2^-126, 1).  The outputs overlap no input.
+ * multiples of 8, heads and weights 16-byte aligned; eps in [2^-126, 1).  The outputs overlap no input.
  */
 int xgen_qk_norm_rope(int dtype, const void *q, int64_t q_stride_batch, int64_t q_stride_seq, int64_t q_stride_head,
                       int64_t q_heads, const void *k, int64_t k_stride_batch, int64_t k_stride_seq,

@@ -12,7 +12,7 @@
 // rounding at the store; layer statistics are two-pass in registers.
 //
 // Layout: a lane holds 8 consecutive values (16 bytes), a power of two of lanes a head, so its reductions are
-// lane shuffles; a wave takes kGroups such groups of heads of one token.  The halves' partner is another
+// lane shuffles; a wave takes GROUPS such groups of heads of one token.  The halves' partner is another
 // lane's chunk (or, where the pairs are no multiple of 8, read again from memory).
 #include <utility>
 
@@ -24,7 +24,11 @@ namespace xgen {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kGroups = 4;
+
+// Heads that a wave takes, in groups of 64 / LANES: four groups past the caches (15,624 tokens of 112 heads of 128: 172 us,
+// 175 with two), one in calls of few groups (64 tokens of those: 3.7 us against 3.9 with two; 128 tokens, 3,584
+// groups: 4.9 against 4.7), two in the others (2,000 tokens: 31 us, 35 with one).
+constexpr int64_t kFewGroups = 2560;
 
 // Where a chunk's partners come from: halves by whole chunks, side by side, or halves of any length.
 enum Pairing { kHalves = 0, kBeside = 1, kHalvesAny = 2 };
@@ -34,14 +38,15 @@ struct Heads {
   int64_t sb, ss, sh;  // bytes
   const void *w;
   uint8_t *out;
-  int heads, groups;   // groups: of 64 / lanes-per-head heads
+  int heads;
 };
 
 struct RotateArgs {
   Heads t[2];          // queries, keys
   int64_t tokens;
   FastDiv seq;         // token t = b * seq + s
-  FastDiv waves;       // wave i = token * waves + part: a token's groups, kGroups a wave
+  FastDiv waves;       // wave i = token * waves + part: GROUPS groups of 64 / LANES heads
+  int query_waves;     // the parts that are queries'
   int dim, pairs;
   int norm, weight_dtype;
   bool aligned_tables;
@@ -76,49 +81,65 @@ __device__ __forceinline__ float load_weight(const void *w, int dtype, int i) {
   return (float)static_cast<const _Float16 *>(w)[i];
 }
 
-template <int DT, int LANES, int PAIRING>
+// Eight weights from a multiple of 8 on.
+__device__ __forceinline__ void load_weights(const void *w, int dtype, int i, float (&v)[8]) {
+  if (dtype == XGEN_DTYPE_F32) {
+    const f32x4 *q = reinterpret_cast<const f32x4 *>(static_cast<const float *>(w) + i);
+    const f32x4 a = q[0], b = q[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+  } else {
+    const u32x4 c = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(w) + i);
+    if (dtype == XGEN_DTYPE_BF16) unpack8<XGEN_DTYPE_BF16>(c, v);
+    else unpack8<XGEN_DTYPE_F16>(c, v);
+  }
+}
+
+template <int DT, int LANES, int PAIRING, int GROUPS, bool PAST>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs p) {
   const int lane = threadIdx.x & 63;
   const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + (threadIdx.x >> 6)));
   const uint32_t token = fast_div(id, p.waves);
   if (token >= p.tokens) return;
-  const int first = (int)(id - token * p.waves.d) * kGroups;
+  // (queries' waves first: a wave's groups are of one set)
+  const int part = (int)(id - token * p.waves.d);
+  const bool keys = part >= p.query_waves;
+  const Heads &t = p.t[keys];
   const uint32_t b = fast_div(token, p.seq), s = token - b * p.seq.d;
   constexpr int kHeads = 64 / LANES;  // heads of a group
   const int chunk = lane & (LANES - 1), sub = lane / LANES;
   const int e0 = chunk * 8;
   const bool in = e0 < p.dim;
-  const int groups = p.t[0].groups + p.t[1].groups;
+  const int head0 = (keys ? part - p.query_waves : part) * (GROUPS * kHeads);
 
   // this lane's chunks, all in flight at once
-  u32x4 c[kGroups];
-  const uint8_t *src[kGroups];
+  const uint8_t *src = t.x + b * t.sb + s * t.ss + (int64_t)(head0 + sub) * t.sh + e0 * 2;
+  u32x4 c[GROUPS];
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    const bool keys = first + g >= p.t[0].groups;
-    const Heads &t = p.t[keys];
-    const int head = (first + g - (keys ? p.t[0].groups : 0)) * kHeads + sub;
+  for (int g = 0; g < GROUPS; ++g) {
     c[g] = u32x4{0, 0, 0, 0};
-    src[g] = nullptr;
-    if (first + g < groups && head < t.heads && in) {
-      src[g] = t.x + b * t.sb + s * t.ss + head * t.sh;
-      c[g] = *reinterpret_cast<const u32x4 *>(src[g] + e0 * 2);
-    }
+    if (in && head0 + g * kHeads + sub < t.heads) c[g] = stream_load<PAST>(reinterpret_cast<const u32x4 *>(src + g * kHeads * t.sh));
   }
 
   const int64_t place = p.positions ? p.positions[b * p.position_batch + s] : (int64_t)s;
   const bool known = (uint64_t)place < (uint64_t)p.places;
-  // this lane's values' cosines, and sines with the sign of the partner's product (1 and 0 past the pairs)
-  float co[8], si[8];
+  // place of value e's partner in its head
   const int rotary = 2 * p.pairs;
+  auto partner = [&](int e) {
+    if (e >= rotary) return e;
+    if constexpr (PAIRING == kBeside) return e ^ 1;
+    else return e < p.pairs ? e + p.pairs : e - p.pairs;
+  };
+  // this lane's values' weights on the cosines, and their partners' on the sines with the product's sign (1 and 0 past the pairs)
+  float cw[8], sw[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) co[i] = 1.0f, si[i] = 0.0f;
+  for (int i = 0; i < 8; ++i) cw[i] = 1.0f, sw[i] = 0.0f;
   if (known && e0 < rotary) {
     const float *pc = p.cos + place * p.pairs, *ps = p.sin + place * p.pairs;
     if (PAIRING == kBeside && p.aligned_tables) {  // four pairs (their number a multiple of 4)
       const f32x4 a = *reinterpret_cast<const f32x4 *>(pc + e0 / 2), d = *reinterpret_cast<const f32x4 *>(ps + e0 / 2);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) co[i] = a[i / 2], si[i] = i & 1 ? d[i / 2] : -d[i / 2];
+      for (int i = 0; i < 8; ++i) cw[i] = a[i / 2], sw[i] = i & 1 ? d[i / 2] : -d[i / 2];
     } else if (PAIRING == kHalves && p.aligned_tables) {  // eight pairs' first or second values
       const bool second = e0 >= p.pairs;
       const int i0 = second ? e0 - p.pairs : e0;
@@ -126,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs p) {
       for (int h = 0; h < 2; ++h) {
         const f32x4 a = *reinterpret_cast<const f32x4 *>(pc + i0 + h * 4), d = *reinterpret_cast<const f32x4 *>(ps + i0 + h * 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) co[h * 4 + i] = a[i], si[h * 4 + i] = second ? d[i] : -d[i];
+        for (int i = 0; i < 4; ++i) cw[h * 4 + i] = a[i], sw[h * 4 + i] = second ? d[i] : -d[i];
       }
     } else {
 #pragma unroll
@@ -134,37 +155,38 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs p) {
         if (e0 + i < rotary) {
           const bool second = PAIRING == kBeside ? i & 1 : e0 + i >= p.pairs;
           const int at = PAIRING == kBeside ? (e0 + i) / 2 : second ? e0 + i - p.pairs : e0 + i;
-          co[i] = pc[at], si[i] = second ? ps[at] : -ps[at];
+          cw[i] = pc[at], sw[i] = second ? ps[at] : -ps[at];
         }
     }
   }
+  if (t.w && in) {
+    float w[8];
+    load_weights(t.w, p.weight_dtype, e0, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cw[i] *= w[i];
+    if constexpr (PAIRING == kBeside) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sw[i] *= w[i ^ 1];
+    } else if constexpr (PAIRING == kHalves) {
+      load_weights(t.w, p.weight_dtype, partner(e0), w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sw[i] *= w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sw[i] *= load_weight(t.w, p.weight_dtype, partner(e0 + i));
+    }
+  }
 
-  // place of value e's partner in its head
-  auto partner = [&](int e) {
-    if (e >= rotary) return e;
-    if constexpr (PAIRING == kBeside) return e ^ 1;
-    else return e < p.pairs ? e + p.pairs : e - p.pairs;
-  };
   // the lane whose chunk holds this chunk's partners (kHalves; its own past the pairs)
   const int other = PAIRING == kHalves ? lane + (partner(e0) - e0) / 8 : lane;
   const float inv_dim = 1.0f / (float)p.dim;
-  float cw[8], sw[8];
+  uint8_t *out = t.out + (((int64_t)token * t.heads + head0 + sub) * p.dim + e0) * 2;
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    if (first + g >= groups) break;  // (uniform)
-    const bool keys = first + g >= p.t[0].groups;
-    const Heads &t = p.t[keys];
-    if (g == 0 || first + g == p.t[0].groups) {  // the set's weights on the token's angles
-#pragma unroll
-      for (int i = 0; i < 8; ++i) cw[i] = co[i], sw[i] = si[i];
-      if (t.w && in) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          cw[i] *= load_weight(t.w, p.weight_dtype, e0 + i);
-          sw[i] *= load_weight(t.w, p.weight_dtype, partner(e0 + i));
-        }
-      }
-    }
+  for (int g = 0; g < GROUPS; ++g) {
+    // (a group's values are formed behind the one before's: all at once take three times the registers)
+    __builtin_amdgcn_sched_barrier(0);
+    if (head0 + g * kHeads >= t.heads) break;  // (uniform)
+    const bool mine = in && head0 + g * kHeads + sub < t.heads;
     float v[8], o[8];
     unpack8<DT>(c[g], v);
     if constexpr (PAIRING == kBeside) {
@@ -176,10 +198,12 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs p) {
       for (int i = 0; i < 4; ++i) x[i] = (uint32_t)__shfl((int)c[g][i], other);
       unpack8<DT>(x, o);
     } else {
+      const uint8_t *head = src + g * kHeads * t.sh - e0 * 2;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = src[g] && e0 + i < rotary ? load_value<DT>(src[g] + partner(e0 + i) * 2) : 0.0f;
+      for (int i = 0; i < 8; ++i) o[i] = mine && e0 + i < rotary ? load_value<DT>(head + partner(e0 + i) * 2) : 0.0f;
     }
-    float mean = 0.0f, scale = 1.0f;
+    // (an unknown place: NaN throughout)
+    float mean = 0.0f, scale = known ? 1.0f : __builtin_nanf("");
     if (p.norm != XGEN_NORM_NONE) {
       if (p.norm == XGEN_NORM_LAYER) {
         float sum = 0.0f;
@@ -194,43 +218,49 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(v[i], v[i], sum);
       }
-      scale = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<LANES>(sum), inv_dim, p.eps));
+      scale *= __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<LANES>(sum), inv_dim, p.eps));
     }
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       // (past the pairs the partner's product is none: a partner of inf would make it NaN)
       const float turn = e0 + i < rotary ? o[i] * sw[i] : 0.0f;
-      y[i] = known ? __builtin_fmaf(v[i], cw[i], turn) * scale : __builtin_nanf("");
+      y[i] = __builtin_fmaf(v[i], cw[i], turn) * scale;
     }
-    if (src[g]) {
-      const int head = (first + g - (keys ? p.t[0].groups : 0)) * kHeads + sub;
+    if (mine) {
       u32x4 r;
       if constexpr (DT == XGEN_DTYPE_BF16)
         r = u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};
       else
         r = u32x4{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]), pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7])};
-      *reinterpret_cast<u32x4 *>(t.out + (((int64_t)token * t.heads + head) * p.dim + e0) * 2) = r;
+      stream_store<PAST>(reinterpret_cast<u32x4 *>(out + g * kHeads * p.dim * 2), r);
     }
   }
 }
 
+template <int DT, int LANES, int PAIRING>
+void launch_rotate(const RotateArgs &p, int groups, bool past, unsigned blocks, hipStream_t stream) {
+  if (groups == 1) rotate_kernel<DT, LANES, PAIRING, 1, false><<<blocks, kThreads, 0, stream>>>(p);
+  else if (past) rotate_kernel<DT, LANES, PAIRING, 4, true><<<blocks, kThreads, 0, stream>>>(p);
+  else rotate_kernel<DT, LANES, PAIRING, 2, false><<<blocks, kThreads, 0, stream>>>(p);
+}
+
 template <int DT, int LANES>
-void launch_rotate(const RotateArgs &p, int pairing, unsigned blocks, hipStream_t stream) {
-  if (pairing == kHalves) rotate_kernel<DT, LANES, kHalves><<<blocks, kThreads, 0, stream>>>(p);
-  else if (pairing == kBeside) rotate_kernel<DT, LANES, kBeside><<<blocks, kThreads, 0, stream>>>(p);
-  else rotate_kernel<DT, LANES, kHalvesAny><<<blocks, kThreads, 0, stream>>>(p);
+void launch_rotate(const RotateArgs &p, int pairing, int groups, bool past, unsigned blocks, hipStream_t stream) {
+  if (pairing == kHalves) launch_rotate<DT, LANES, kHalves>(p, groups, past, blocks, stream);
+  else if (pairing == kBeside) launch_rotate<DT, LANES, kBeside>(p, groups, past, blocks, stream);
+  else launch_rotate<DT, LANES, kHalvesAny>(p, groups, past, blocks, stream);
 }
 
 template <int DT>
-void launch_rotate(const RotateArgs &p, int lanes, int pairing, unsigned blocks, hipStream_t stream) {
+void launch_rotate(const RotateArgs &p, int lanes, int pairing, int groups, bool past, unsigned blocks, hipStream_t stream) {
   switch (lanes) {
-    case 2: return launch_rotate<DT, 2>(p, pairing, blocks, stream);
-    case 4: return launch_rotate<DT, 4>(p, pairing, blocks, stream);
-    case 8: return launch_rotate<DT, 8>(p, pairing, blocks, stream);
-    case 16: return launch_rotate<DT, 16>(p, pairing, blocks, stream);
-    case 32: return launch_rotate<DT, 32>(p, pairing, blocks, stream);
-    default: return launch_rotate<DT, 64>(p, pairing, blocks, stream);
+    case 2: return launch_rotate<DT, 2>(p, pairing, groups, past, blocks, stream);
+    case 4: return launch_rotate<DT, 4>(p, pairing, groups, past, blocks, stream);
+    case 8: return launch_rotate<DT, 8>(p, pairing, groups, past, blocks, stream);
+    case 16: return launch_rotate<DT, 16>(p, pairing, groups, past, blocks, stream);
+    case 32: return launch_rotate<DT, 32>(p, pairing, groups, past, blocks, stream);
+    default: return launch_rotate<DT, 64>(p, pairing, groups, past, blocks, stream);
   }
 }
 
@@ -317,24 +347,29 @@ extern "C" int xgen_qk_norm_rope(int dtype, const void *q, int64_t q_stride_batc
   for (const auto &t : {std::make_pair(q_heads ? q : nullptr, q_heads ? q_out : nullptr),
                         std::make_pair(k_heads ? k : nullptr, k_heads ? k_out : nullptr)})
     if (!aligned16(t.first) || !aligned16(t.second)) return fail(XGEN_ERR_UNSUPPORTED, "%s: heads must be 16-byte aligned", fn);
+  if ((q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)))
+    return fail(XGEN_ERR_UNSUPPORTED, "%s: weights must be 16-byte aligned", fn);
   if ((q_heads && (q_stride_batch % 8 || q_stride_seq % 8 || q_stride_head % 8)) ||
       (k_heads && (k_stride_batch % 8 || k_stride_seq % 8 || k_stride_head % 8)))
     return fail(XGEN_ERR_UNSUPPORTED, "%s: strides must be multiples of 8", fn);
   int lanes = 2;
   while (lanes * 8 < dim) lanes *= 2;
   const int64_t per = 64 / lanes, groups_q = (q_heads + per - 1) / per, groups_k = (k_heads + per - 1) / per;
-  const int64_t waves = (groups_q + groups_k + kGroups - 1) / kGroups;
+  const bool past = batch * seq * (q_heads + k_heads) * dim * 4 > kLastLevelCacheBytes;  // read and written
+  const int groups = past ? 4 : batch * seq * (groups_q + groups_k) <= kFewGroups ? 1 : 2;
+  const int64_t waves_q = (groups_q + groups - 1) / groups, waves = waves_q + (groups_k + groups - 1) / groups;
   if (q_heads >= (1 << 24) || k_heads >= (1 << 24) || batch >= (1ll << 31) || seq >= (1ll << 31) ||
       batch * seq >= (1ll << 31) || batch * seq * waves >= (1ll << 31) - kWaves)
     return fail(XGEN_ERR_UNSUPPORTED, "%s: too many tokens or heads", fn);
   RotateArgs p;
   p.t[0] = {static_cast<const uint8_t *>(q), q_stride_batch * 2, q_stride_seq * 2, q_stride_head * 2, q_weight,
-            static_cast<uint8_t *>(q_out), (int)q_heads, (int)groups_q};
+            static_cast<uint8_t *>(q_out), (int)q_heads};
   p.t[1] = {static_cast<const uint8_t *>(k), k_stride_batch * 2, k_stride_seq * 2, k_stride_head * 2, k_weight,
-            static_cast<uint8_t *>(k_out), (int)k_heads, (int)groups_k};
+            static_cast<uint8_t *>(k_out), (int)k_heads};
   p.tokens = batch * seq;
   p.seq = make_fastdiv((uint32_t)seq);
   p.waves = make_fastdiv((uint32_t)waves);
+  p.query_waves = (int)waves_q;
   p.dim = (int)dim;
   p.pairs = (int)pairs;
   p.norm = norm_kind;
@@ -348,8 +383,8 @@ extern "C" int xgen_qk_norm_rope(int dtype, const void *q, int64_t q_stride_batc
   p.position_batch = position_stride_batch;
   const int pairing = interleaved ? kBeside : pairs % 8 == 0 ? kHalves : kHalvesAny;
   const unsigned blocks = (unsigned)((batch * seq * waves + kWaves - 1) / kWaves);
-  if (dtype == XGEN_DTYPE_BF16) launch_rotate<XGEN_DTYPE_BF16>(p, lanes, pairing, blocks, stream);
-  else launch_rotate<XGEN_DTYPE_F16>(p, lanes, pairing, blocks, stream);
+  if (dtype == XGEN_DTYPE_BF16) launch_rotate<XGEN_DTYPE_BF16>(p, lanes, pairing, groups, past, blocks, stream);
+  else launch_rotate<XGEN_DTYPE_F16>(p, lanes, pairing, groups, past, blocks, stream);
   return launch_status(fn);
 }
 

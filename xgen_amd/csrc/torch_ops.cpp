@@ -765,7 +765,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor &q_in, const Tensor &k_in, 
     return ok || t.numel() == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
   };
   const Tensor q = heads(q_in), k = heads(k_in), cos = cos_in.contiguous(), sin = sin_in.contiguous();
-  Tensor wq = q_weight ? q_weight->contiguous() : Tensor(), wk = k_weight ? k_weight->contiguous() : Tensor();
+  Tensor wq = optional_flat(q_weight), wk = optional_flat(k_weight);
   if (wq.defined() && wk.defined() && wq.scalar_type() != wk.scalar_type()) {  // one dtype for both: the wider, exactly
     wq = wq.to(at::kFloat);
     wk = wk.to(at::kFloat);
