@@ -158,18 +158,16 @@ void gemm_tile_kernel(GemmArgs p) {
   // --- fragments: [register buffer = sub-stage][k step][fragment] ---
   const int row_x = wm * 32 * FM + (lane & 31), row_w = wn * 32 * FN + (lane & 31);
   frag_t xf[2][KS][FM], wf[2][KS][FN];
-  [[maybe_unused]] uint32_t xsc[2][kMx ? FM : 1], wsc[2][kMx ? FN : 1];
+  // MXFP4: this lane's scales per fragment, weights first; sub-stage 1 has a copy, as sub-stage 0's are written under it
+  [[maybe_unused]] uint32_t sc[2][kMx ? FN + FM : 1];
+  [[maybe_unused]] auto read_scale = [&](uint32_t slot, int f) {
+    const uint8_t *rows = smem + C::kScaleBase + slot / C::kSlotBytes * C::kScaleSlot;
+    const uint8_t *row = f < FN ? rows + C::kScaleA * 1024 + (row_w + f * 32) * 8 : rows + (row_x + (f - FN) * 32) * 8;
+    return *reinterpret_cast<const uint32_t *>(row + (lane >> 5) * 4);
+  };
   uint32_t rd_slot = 0;  // LDS offset of the pair being multiplied
-  // fragment r of sub-stage b, weights first (sslot: the slot's place in the scales' ring)
-  auto read_frag = [&](int b, uint32_t slot, [[maybe_unused]] uint32_t sslot, int r) {
+  auto read_frag = [&](int b, uint32_t slot, int r) {  // fragment r of sub-stage b, weights first
     const int ks = r / (FM + FN), f = r % (FM + FN);
-    if constexpr (kMx) {  // with step 0's fragment, the row's two scale bytes of the sub-stage
-      if (ks == 0) {
-        const uint32_t sc = C::kScaleBase + sslot + (lane >> 5) * 4 + b * 2;
-        if (f < FN) wsc[b][f] = *reinterpret_cast<const uint16_t *>(smem + sc + C::kScaleA * 1024 + (row_w + f * 32) * 8);
-        else xsc[b][f - FN] = *reinterpret_cast<const uint16_t *>(smem + sc + (row_x + (f - FN) * 32) * 8);
-      }
-    }
     if (f < FN) wf[b][ks][f] = load_pair<KIND>(smem + slot + C::kM * 128, row_w + f * 32, b, ks, lane);
     else xf[b][ks][f - FN] = load_pair<KIND>(smem + slot, row_x + (f - FN) * 32, b, ks, lane);
   };
@@ -189,7 +187,6 @@ void gemm_tile_kernel(GemmArgs p) {
     constexpr int b = decltype(B)::value;
     constexpr bool load = decltype(LOAD)::value, read = decltype(READ)::value;
     if constexpr (b == 1 && load) issue_begin();
-    const uint32_t next_sslot = kMx ? next_slot / C::kSlotBytes * C::kScaleSlot : 0;
     // the MFMAs are volatile asm statements: the loads written between them stay there
     // (the exact kind widens each activation fragment once per sub-stage and, weights
     // outermost, each weight fragment once too)
@@ -208,8 +205,18 @@ void gemm_tile_kernel(GemmArgs p) {
         MfmaA<KIND>::mma(acc[i][j], wf[b][ks][i], xw[0]);
       } else if constexpr (kMx) {
         const int j = (s / FN) % FM, i = s % FN;
-        if (ks == 0) MfmaA<KIND>::template mma<0>(acc[i][j], wf[b][ks][i], xf[b][ks][j], wsc[b][i], xsc[b][j]);
-        else MfmaA<KIND>::template mma<1>(acc[i][j], wf[b][ks][i], xf[b][ks][j], wsc[b][i], xsc[b][j]);
+        // (s is a constant once unrolled: one of the branches stays)
+        if (ks == 0) MfmaA<KIND>::template mma<2 * b>(acc[i][j], wf[b][ks][i], xf[b][ks][j], sc[b][i], sc[b][FN + j]);
+        else MfmaA<KIND>::template mma<2 * b + 1>(acc[i][j], wf[b][ks][i], xf[b][ks][j], sc[b][i], sc[b][FN + j]);
+        if constexpr (b == 1 && read) {  // the next pair's scales
+#pragma unroll
+          for (int f = spread_first(s, FN + FM, kMfmas); f < spread_first(s + 1, FN + FM, kMfmas); ++f) sc[0][f] = read_scale(next_slot, f);
+        }
+        if constexpr (b == 0) {
+#pragma unroll
+          for (int f = spread_first(s, FN + FM, kMfmas); f < spread_first(s + 1, FN + FM, kMfmas); ++f)
+            asm volatile("v_mov_b32 %0, %1" : "=v"(sc[1][f]) : "v"(sc[0][f]));
+        }
       } else {
         const int j = (s / FN) % FM, i = s % FN;
         MfmaA<KIND>::mma(acc[i][j], wf[b][ks][i], xf[b][ks][j]);
@@ -217,7 +224,7 @@ void gemm_tile_kernel(GemmArgs p) {
       if constexpr (read) {
 #pragma unroll
         for (int r = spread_first(s, kFrags, kMfmas); r < spread_first(s + 1, kFrags, kMfmas); ++r)
-          read_frag(b ^ 1, next_slot, next_sslot, r);
+          read_frag(b ^ 1, next_slot, r);
       }
       if constexpr (load && kSpread) {
         // sub-stage 1 takes the first half of a pair's loads, the next sub-stage 0 the rest
@@ -229,6 +236,8 @@ void gemm_tile_kernel(GemmArgs p) {
         for (int q = spread_first(s, C::kLoads, kMfmas); q < spread_first(s + 1, C::kLoads, kMfmas); ++q) issue_load(q);
       }
     }
+    // (the copies, two wait states ahead of the next sub-stage's first MFMA: the compiler cannot see that it reads them)
+    if constexpr (kMx && b == 0) asm volatile("s_nop 1");
     if constexpr (load && b == (kSpread ? 0 : 1)) issue_end();
   };
   typedef std::integral_constant<int, 0> B0;
@@ -247,7 +256,11 @@ void gemm_tile_kernel(GemmArgs p) {
   wait_vmcnt<(SLOTS - 1) * kPairLoads - (kSpread ? C::kLoads / 2 : 0)>();
   lds_barrier();
 #pragma unroll
-  for (int r = 0; r < kFrags; ++r) read_frag(0, 0, 0, r);
+  for (int r = 0; r < kFrags; ++r) read_frag(0, 0, r);
+  if constexpr (kMx) {
+#pragma unroll
+    for (int f = 0; f < FN + FM; ++f) sc[0][f] = read_scale(0, f);
+  }
 
   // pairs past K are zeros: the ring is filled once at least
   const int pairs = (p.K + 127) / 128 > SLOTS ? (p.K + 127) / 128 : SLOTS;

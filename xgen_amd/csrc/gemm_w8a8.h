@@ -1,4 +1,4 @@
-// Pieces shared by the W8A8 and MXFP4 GEMM kernels (gemm_w8a8.hip: one persistent workgroup
+// Pieces shared by the W8A8 and MXFP4 GEMM kernels (gemm_w8a8.hip, mxfp4_gemm.hip: one persistent workgroup
 // per CU on 256 x 256 tiles; gemm_tile.hip: smaller tiles): the arguments, the
 // operand kinds' MFMA wrappers, the LDS-DMA load and the LDS row layout.
 #pragma once
@@ -67,6 +67,9 @@ int choose_gemm_tile(int kind, int64_t M, int64_t N, int64_t K, bool gated, bool
 // Launches the call on that tile.  g: filled as for the 256 x 256 kernel.
 void launch_gemm_tile(int kind, int tile, const GemmArgs &g, hipStream_t stream);
 
+// Launches an MXFP4 call on 256 x 256 tiles (mxfp4_gemm.hip).
+void launch_mx4_gemm(const GemmArgs &g, hipStream_t stream);
+
 // Operand traits per kind: accumulator and fragment types (one fragment = 32
 // rows of one 64-byte K step, as the fragment reads deliver them), MFMA steps per
 // 64-byte K step, 16-byte LDS reads per fragment, accumulator to float.
@@ -110,8 +113,10 @@ struct Mfma<kInt8> {
 };
 
 // MXFP4: fragments lie as INT8's.  Lane half h of a 32x32x64 step holds one block of 32 values per row, and a row's
-// 8 scale bytes of 256 values are ordered (block mod 2) * 4 + block / 2: a lane's four bytes of a pair (its
-// blocks h, h + 2, h + 4, h + 6) are one dword, step s taking byte s.
+// 8 scale bytes of 256 values (a pair of stages) are ordered (block mod 2) * 4 + block / 2: half h's four bytes, of its
+// blocks h, h + 2, h + 4 and h + 6, are one dword, and step s of the pair takes byte s.  (16 x 16 x 128 fragments draw less
+// power: a loop of matrix instructions alone does 7.3 PFLOP/s on random codes against 6.5, 9.6 on zeros either way.  But
+// there are twice as many to issue, and the 256 x 256 kernel on them took 575 us where this one takes 550, mxfp4_gemm.hip.)
 template <>
 struct Mfma<kMx4> {
   typedef f32x16 acc_t;
@@ -215,21 +220,19 @@ struct MfmaA<kInt8> {
     asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, 0" : "=a"(c) : "v"(w), "v"(x));
   }
 };
-// BYTE: the byte of both scale dwords that holds this step's block.
+// STEP: the pair's step of 64 values, whose scales are that byte of both scale registers.
 template <>
 struct MfmaA<kMx4> {
-#define XGEN_MX4(ADDEND, OPSEL) "v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, " ADDEND ", %3, %4 " OPSEL " cbsz:4 blgp:4"
-  template <int BYTE>
+#define XGEN_MX4(OPSEL)                                                                                              \
+  asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 " OPSEL " cbsz:4 blgp:4" : "+a"(c) : "v"(w), "v"(x), \
+               "v"(sw), "v"(sx))
+  template <int STEP>
   static __device__ __forceinline__ void mma(f32x16 &c, const i32x4 &w, const i32x4 &x, uint32_t sw, uint32_t sx) {
-    static_assert(BYTE >= 0 && BYTE < 4, "scale byte");
-    if constexpr (BYTE == 0) asm volatile(XGEN_MX4("%0", "op_sel_hi:[0,0,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
-    else if constexpr (BYTE == 1) asm volatile(XGEN_MX4("%0", "op_sel:[1,1,0] op_sel_hi:[0,0,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
-    else if constexpr (BYTE == 2) asm volatile(XGEN_MX4("%0", "op_sel_hi:[1,1,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
-    else asm volatile(XGEN_MX4("%0", "op_sel:[1,1,0] op_sel_hi:[1,1,0]") : "+a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
-  }
-  // (a tile's first step is byte 0's)
-  static __device__ __forceinline__ void mma0(f32x16 &c, const i32x4 &w, const i32x4 &x, uint32_t sw, uint32_t sx) {
-    asm volatile(XGEN_MX4("0", "op_sel_hi:[0,0,0]") : "=a"(c) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+    static_assert(STEP >= 0 && STEP < 4, "step of a pair");
+    if constexpr (STEP == 0) XGEN_MX4("op_sel_hi:[0,0,0]");
+    else if constexpr (STEP == 1) XGEN_MX4("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+    else if constexpr (STEP == 2) XGEN_MX4("op_sel_hi:[1,1,0]");
+    else XGEN_MX4("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
   }
 #undef XGEN_MX4
 };

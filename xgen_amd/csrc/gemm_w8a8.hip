@@ -10,8 +10,8 @@
 //              matrix-core time of the FP8 instructions, plus the conversions
 //   INT8     : v_mfma_i32_32x32x32_i8      (int8 x int8 -> exact int32)
 //              replaces torch_npu.npu_quant_matmul at x_base/x_base/operator/matmul.py:63-64
-//   MXFP4    : v_mfma_scale_f32_32x32x64_f8f6f4 (e2m1 x e2m1, one e8m0 scale per 32
-//              values of either operand -> fp32), in its own entry (xgen_mxfp4_matmul)
+//
+// (MXFP4 products: checked and split into launches here, on the kernels of mxfp4_gemm.hip and gemm_tile.h.)
 //
 // The FP8 instructions (all shapes, measured on gfx950) do not sum like IEEE
 // fp32: within each group of 8 consecutive K the products are truncated toward
@@ -96,19 +96,6 @@ constexpr int kXposeRow = 136;
 constexpr int kXpose = 32 * kXposeRow;
 constexpr int kXposeBase = kParamBase + kParamSets * kParamBytes;
 constexpr int kLdsBytes = kXposeBase + kWaves * kXpose;  // 154 KB
-// MXFP4: a parameter set is its bias row, and behind the transpose areas each pair slot has the scale bytes of
-// its 256 activation and 256 weight rows, 8 of a row.  One 1 KB load per wave and pair: waves 0 and 1 the
-// activations' halves, 2 and 3 the weights'.
-constexpr int kScaleSlot = 2 * 256 * 8;
-template <int KIND>
-struct Lds {
-  static constexpr bool kMx = KIND == kMx4;
-  static constexpr int kParam = kMx ? 1024 : kParamBytes, kBias = kMx ? 0 : 2048;
-  static constexpr int kXpose0 = kParamBase + kParamSets * kParam;
-  static constexpr int kScale0 = kXpose0 + kWaves * kXpose;
-  static constexpr int kBytes = kScale0 + (kMx ? kPairSlots * kScaleSlot : 0);
-  static_assert(kBytes <= 160 * 1024 && (kMx || kBytes == kLdsBytes), "LDS");
-};
 }  // namespace w4
 
 // 24 wait states after the last MFMAs before any accumulator is read by VALU
@@ -132,9 +119,7 @@ void gemm_w4_kernel(GemmArgs p) {
   constexpr int FM = 4, FN = 4, KS = T::kSteps;
   constexpr int kMfmas = KS * FM * FN;                 // per stage per wave
   constexpr int kReads = T::kReads * KS * (FM + FN);   // ds_read_b128 per stage per wave
-  typedef Lds<KIND> L;
-  constexpr bool kMx = KIND == kMx4;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[L::kBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kLdsBytes];
 
   // --- this workgroup's tiles: a contiguous range per XCD, strided by workgroup ---
   const int ntiles = p.tiles_m * p.tiles_n;
@@ -160,8 +145,8 @@ void gemm_w4_kernel(GemmArgs p) {
       const_cast<float *>(p.sw), (short)0, p.N * 4, kBufferFlags);
   const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<void *>(p.bias), (short)0, p.bias ? p.N * bias_elem : 0, kBufferFlags);
-  const float sa0 = kMx || p.sa_stride ? 0.0f : p.sa[0];  // per-tensor scales
-  const float sw0 = kMx || p.sw_stride ? 0.0f : p.sw[0];
+  const float sa0 = p.sa_stride ? 0.0f : p.sa[0];  // per-tensor scales
+  const float sw0 = p.sw_stride ? 0.0f : p.sw[0];
   // the output rows as a buffer: stores at kOutOfRange are dropped
   const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(p.out, (short)0, (int)p.out_bytes, kBufferFlags);
   // the gated epilogue's residual rows and gate table (reads past them return zeros)
@@ -195,24 +180,11 @@ void gemm_w4_kernel(GemmArgs p) {
   };
   auto issue_begin = [&](int slot) {
     if (dma_k == 0 && dma_h < GP) {  // the tile's epilogue parameters ride with its first pair
-      uint8_t *prm = smem + kParamBase + (dma_i % kParamSets) * L::kParam;
-      if constexpr (!kMx) {
-        if (wave == 0 && p.sa_stride) dma_load16(rsa, prm, (uint32_t)dma_m0 * 4 + lane * 16);
-        if (wave == 1 && p.sw_stride) dma_load16(rsw, prm + 1024, (uint32_t)dma_n0 * 4 + lane * 16);
-      }
+      uint8_t *prm = smem + kParamBase + (dma_i % kParamSets) * kParamBytes;
+      if (wave == 0 && p.sa_stride) dma_load16(rsa, prm, (uint32_t)dma_m0 * 4 + lane * 16);
+      if (wave == 1 && p.sw_stride) dma_load16(rsw, prm + 1024, (uint32_t)dma_n0 * 4 + lane * 16);
       // (without a bias the resource is empty: the row reads as zeros)
-      if (wave == 2) dma_load16(rb, prm + L::kBias, (uint32_t)(dma_n0 * bias_elem) + lane * 16);
-    }
-    if constexpr (kMx) {
-      // the pair's scale bytes: a resource of one 256-value block's rows, empty past K (zeros: 2^-127 times
-      // the zero codes there)
-      const bool act = wave < 2;
-      const bool some = dma_h < GP && dma_k * 128 < p.K;
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint8_t *>(act ? p.xs + dma_k * p.xs_block : p.ws + dma_k * p.ws_block), (short)0,
-          some ? (int)(act ? p.xs_rows : p.ws_rows) : 0, kBufferFlags);
-      dma_load16(rs, smem + L::kScale0 + slot * kScaleSlot + wave * 1024,
-                 (uint32_t)((act ? dma_m0 : dma_n0) + (wave & 1) * 128) * 8 + lane * 16);
+      if (wave == 2) dma_load16(rb, prm + 2048, (uint32_t)(dma_n0 * bias_elem) + lane * 16);
     }
     const int k0 = dma_k * 128;
     const bool live = dma_h < GP;
@@ -252,14 +224,6 @@ void gemm_w4_kernel(GemmArgs p) {
     wf[b][ks][i] = load_pair<KIND>(smem + (s >> 1) * kPairSlotBytes + kPairTile, row_w + i * 32, s & 1, ks, lane);
   };
 
-  // MXFP4: this lane's four scale bytes per fragment row of a pair, [pair slot][fragment]
-  [[maybe_unused]] uint32_t xsc[kMx ? 2 : 1][FM], wsc[kMx ? 2 : 1][FN];
-  auto read_scale = [&](int slot, int f) {  // weights first
-    const uint8_t *sc = smem + L::kScale0 + slot * kScaleSlot + (lane >> 5) * 4;
-    if (f < FN) wsc[slot][f] = *reinterpret_cast<const uint32_t *>(sc + 256 * 8 + (row_w + f * 32) * 8);
-    else xsc[slot][f - FN] = *reinterpret_cast<const uint32_t *>(sc + (row_x + (f - FN) * 32) * 8);
-  };
-
   // defined by each tile's first sub-stage (mma0), read by its epilogue
   typename T::acc_t acc[FN][FM];
 
@@ -272,16 +236,16 @@ void gemm_w4_kernel(GemmArgs p) {
   auto epilogue = [&](auto on_block) {
     int m0, n0;
     tile_origin<256, 256>(t_first + tile_i * wgs_per_xcd, p.tiles_m, p.tiles_n, p.group_m, m0, n0);
-    const uint8_t *prm = smem + kParamBase + (tile_i % kParamSets) * L::kParam;
+    const uint8_t *prm = smem + kParamBase + (tile_i % kParamSets) * kParamBytes;
     const float *psa = reinterpret_cast<const float *>(prm);
     const float *psw = reinterpret_cast<const float *>(prm + 1024);
-    const uint8_t *pb = prm + L::kBias;
+    const uint8_t *pb = prm + 2048;
     // the lane index, opaque: the epilogue's addresses are formed here, not
     // hoisted into registers the stage loop needs
     int el = lane;
     asm volatile("" : "+v"(el));
     const int wrow = el & 31, half = el >> 5;
-    uint8_t *xb = smem + L::kXpose0 + wave * kXpose;
+    uint8_t *xb = smem + kXposeBase + wave * kXpose;
     // this lane's write position (row wrow, 8-byte chunk half + constant), and
     // read position (16 bytes: row (el >> 3) + 8 q, chunk el & 7)
     uint8_t *xw = xb + wrow * kXposeRow + half * 8;
@@ -290,7 +254,7 @@ void gemm_w4_kernel(GemmArgs p) {
     // the per-token scales of this lane's rows, one per j (the same in both halves)
     float sam4[FM];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) sam4[j] = kMx ? 1.0f : p.sa_stride ? psa[wm * kWaveRows + j * 32 + wrow] : sa0;
+    for (int j = 0; j < FM; ++j) sam4[j] = p.sa_stride ? psa[wm * kWaveRows + j * 32 + wrow] : sa0;
     // The read-back of step (h, j) is stored during step (h, j) + 1, after that
     // step's writes to the same transpose rows: the reads were issued first, and
     // a wave's LDS operations complete in order, so they return step (h, j)'s
@@ -339,7 +303,7 @@ void gemm_w4_kernel(GemmArgs p) {
       // so they issue together and are waited for once)
       f32x4 swr[2][4], bir[2][4];
       const int nl0 = wn * kWaveRows + 2 * h * 32 + half * 4;  // + ii*32 + gq*8
-      if (!kMx && p.sw_stride) {
+      if (p.sw_stride) {
 #pragma unroll
         for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
@@ -407,8 +371,7 @@ void gemm_w4_kernel(GemmArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float a = T::to_f32(acc[i][j][gq * 4 + e]);
-              if constexpr (kMx) y[e] = a + bir[ii][gq][e];
-              else y[e] = __builtin_fmaf(a, sam * swr[ii][gq][e], bir[ii][gq][e]);
+              y[e] = __builtin_fmaf(a, sam * swr[ii][gq][e], bir[ii][gq][e]);
               if constexpr (ACT == XGEN_ACT_GELU_TANH) y[e] = gelu_tanh(round_out<OUT_DT>(y[e]));
             }
             // row wrow, 8-byte chunk ii*8 + gq*2 + half
@@ -513,19 +476,9 @@ void gemm_w4_kernel(GemmArgs p) {
         if (i == 0) xw = MfmaA<KIND>::widen_x(xf[cb][ks][j]);
         if (fresh && ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[cb][ks][i], xw);
         else MfmaA<KIND>::mma(acc[i][j], wf[cb][ks][i], xw);
-      } else if constexpr (kMx) {
-        // (s is a constant once unrolled: one of the branches stays)
-        const uint32_t sw = wsc[u >> 1][i], sx = xsc[u >> 1][j];
-        if (fresh && ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[cb][ks][i], xf[cb][ks][j], sw, sx);
-        else if (ks == 0) MfmaA<KIND>::template mma<cb * 2>(acc[i][j], wf[cb][ks][i], xf[cb][ks][j], sw, sx);
-        else MfmaA<KIND>::template mma<cb * 2 + 1>(acc[i][j], wf[cb][ks][i], xf[cb][ks][j], sw, sx);
       } else {
         if (fresh && ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[cb][ks][i], xf[cb][ks][j]);
         else MfmaA<KIND>::mma(acc[i][j], wf[cb][ks][i], xf[cb][ks][j]);
-      }
-      if constexpr (kMx && read && odd) {  // the next pair's scales, with its first fragments
-#pragma unroll
-        for (int f = spread_first(s, FM + FN, kMfmas); f < spread_first(s + 1, FM + FN, kMfmas); ++f) read_scale(ns >> 1, f);
       }
       if constexpr (read) {
 #pragma unroll
@@ -545,10 +498,6 @@ void gemm_w4_kernel(GemmArgs p) {
   };
   // stage 0's fragments (slot 0, register buffer 0)
   auto read_first = [&]() {
-    if constexpr (kMx) {
-#pragma unroll
-      for (int f = 0; f < FM + FN; ++f) read_scale(0, f);
-    }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -566,13 +515,8 @@ void gemm_w4_kernel(GemmArgs p) {
     epilogue([&](int i, int j, int b) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if constexpr (kMx) {
-          if (ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[0][ks][i], xf[0][ks][j], wsc[0][i], xsc[0][j]);
-          else MfmaA<KIND>::template mma<1>(acc[i][j], wf[0][ks][i], xf[0][ks][j], wsc[0][i], xsc[0][j]);
-        } else {
-          if (ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
-          else MfmaA<KIND>::mma(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
-        }
+        if (ks == 0) MfmaA<KIND>::mma0(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
+        else MfmaA<KIND>::mma(acc[i][j], wf[0][ks][i], xf[0][ks][j]);
       }
       (void)b;
     });
@@ -604,7 +548,7 @@ void gemm_w4_kernel(GemmArgs p) {
 #pragma unroll
     for (int q = 0; q < kLoadsPerPair; ++q) issue_load(is, 1, q);
     issue_end();
-    wait_vmcnt<kLoadsPerPair + (kMx ? 1 : 0)>();
+    wait_vmcnt<kLoadsPerPair>();
     lds_barrier();
     read_first();
   }
@@ -646,11 +590,6 @@ void launch_gemm_w4(const GemmArgs &a, bool acc_out, hipStream_t stream) {
   const dim3 grid = gemm_grid(a), block(w4::kThreads);
   if (acc_out) gemm_w4_kernel<KIND, ACT, OUT_DT, true, false><<<grid, block, 0, stream>>>(a);
   else gemm_w4_kernel<KIND, ACT, OUT_DT, false, false><<<grid, block, 0, stream>>>(a);
-}
-
-template <int KIND, int ACT, int OUT_DT>
-void launch_gemm_plain(const GemmArgs &a, hipStream_t stream) {
-  gemm_w4_kernel<KIND, ACT, OUT_DT, false, false><<<gemm_grid(a), dim3(w4::kThreads), 0, stream>>>(a);
 }
 
 template <int KIND>
@@ -823,11 +762,7 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   }
   const bool with_acc = acc_out != nullptr;
   if constexpr (kMx) {
-    if (gated) launch_gemm_w4_gated<KIND>(g, stream);
-    else if (activation == XGEN_ACT_NONE && out_dtype == XGEN_DTYPE_BF16) launch_gemm_plain<KIND, XGEN_ACT_NONE, XGEN_DTYPE_BF16>(g, stream);
-    else if (activation == XGEN_ACT_NONE) launch_gemm_plain<KIND, XGEN_ACT_NONE, XGEN_DTYPE_F16>(g, stream);
-    else if (out_dtype == XGEN_DTYPE_BF16) launch_gemm_plain<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_BF16>(g, stream);
-    else launch_gemm_plain<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_F16>(g, stream);
+    launch_mx4_gemm(g, stream);
   } else if (gated) {
     // (the gated entry takes the FP8 and INT8 kinds only: no exact-kind instance)
     if constexpr (KIND != kFp8Exact) launch_gemm_w4_gated<KIND>(g, stream);
