@@ -51,8 +51,8 @@ constexpr TileCost kTileCosts[4][kTiles + 1] = {
     {{0.266f, 0.0f, 4.0f}, {0.363f, 0.0f, 3.9f}, {0.367f, 2.2f, 1.5f}, {0.492f, 3.0f, 1.2f}, {0.771f, 4.7f, 0.0f},
      {1.06f, 4.8f, 0.0f}, {1.35f, 6.4f, 0.0f}, {1.92f, 7.8f, 0.0f}, {2.49f, 7.7f, 0.0f}},
     // MXFP4
-    {{0.203f, 0.1f, 3.1f}, {0.319f, 0.0f, 3.7f}, {0.242f, 2.1f, 1.3f}, {0.39f, 1.3f, 3.3f}, {0.503f, 3.9f, 1.8f},
-     {0.668f, 5.2f, 1.8f}, {0.751f, 7.3f, 0.0f}, {1.18f, 8.5f, 0.0f}, {1.54f, 6.7f, 0.1f}},
+    {{0.247f, 1.4f, 1.8f}, {0.363f, 1.9f, 1.2f}, {0.305f, 2.1f, 1.3f}, {0.418f, 3.2f, 0.3f}, {0.56f, 3.9f, 0.2f},
+     {0.711f, 5.2f, 0.2f}, {0.812f, 6.7f, 0.0f}, {1.26f, 8.0f, 1.6f}, {1.37f, 6.4f, 0.9f}},
 };
 // The 256 x 256 kernel keeps a call unless a smaller tile is put 4% below it.  On short K, where
 // the sums put its epilogue too high, 10%: up to K = 512, and against the tiles from 128 x 192 on up
@@ -63,7 +63,10 @@ constexpr TileCost kTileCosts[4][kTiles + 1] = {
 // stores its accumulators stores three times the bytes, on the 256-row tiles all at the end: 15% for them (at
 // the lines above, 15,624 x 5,376 x 384 exact: 228 us on 256 x 192, 148 on the large kernel, and 44
 // of 1,776 calls more than 3% slower than on it; so 18, most of them under K = 1,024, 17% at most).
-float keep_large(int tile, int64_t K, bool gated, bool accumulators) {
+// MXFP4 calls 4% throughout (its figures are from 78 shapes, up to 14,336 x 5,376: the choice is within 0.2% of the
+// best tile on the average; by INT8's figures, with which its kernels began, 1.25%).
+float keep_large(int kind, int tile, int64_t K, bool gated, bool accumulators) {
+  if (kind == kMx4) return 0.96f;
   if (accumulators && kTileSizes[tile].m == 256) return 0.85f;
   const int64_t short_k = kTileSizes[tile].m * kTileSizes[tile].n >= 128 * 192 ? 1024 : 512;
   return !gated && K <= short_k ? 0.90f : 0.96f;
@@ -74,8 +77,8 @@ float tile_cost(int kind, int tile, int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = ((M + t.m - 1) / t.m) * ((N + t.n - 1) / t.n);
   const int64_t cus = device_cu_count();
   const float rounds = (float)((tiles + cus - 1) / cus);
-  // (the 256 x 256 kernel takes pairs two at a time)
-  const int64_t steps = tile == kTiles ? (K + 255) / 256 * 2 : (K + 127) / 128;
+  // (the 256 x 256 kernel of the W8A8 kinds takes pairs two at a time)
+  const int64_t steps = tile == kTiles && kind != kMx4 ? (K + 255) / 256 * 2 : (K + 127) / 128;
   const float pairs = (float)(steps > t.slots ? steps : t.slots);
   const TileCost c = kTileCosts[kind][tile];
   return c.start + rounds * (pairs * c.per_pair + c.per_tile);
@@ -115,7 +118,7 @@ int choose_gemm_tile(int kind, int64_t M, int64_t N, int64_t K, bool gated, bool
   float cost = large;
   for (int t = 0; t < kTiles; ++t) {
     const float c = tile_cost(kind, t, M, N, K);
-    if (c < cost && c < keep_large(t, K, gated, accumulators) * large) best = t, cost = c;
+    if (c < cost && c < keep_large(kind, t, K, gated, accumulators) * large) best = t, cost = c;
   }
   return best;
 }
