@@ -63,7 +63,7 @@ extern "C" {
 
 /* GEMM epilogue activations */
 #define XGEN_ACT_NONE 0
-#define XGEN_ACT_GELU_TANH 1 /* out = bf16(gelu_tanh(bf16(linear))) */
+#define XGEN_ACT_GELU_TANH 1 /* out = bf16(gelu_tanh(bf16(linear))); xgen_mxfp4_matmul: bf16(gelu_tanh(linear)) */
 
 /* expert router: scoring functions, and the largest expert and choice counts */
 #define XGEN_ROUTE_SOFTMAX 0
@@ -570,8 +570,8 @@ int xgen_mxfp4_dequantize(const void *codes, int64_t ld_codes, const void *scale
 /*
  * Product of MXFP4 rows, as xgen_scaled_mm_fp8 of 8-bit ones (no counterpart in the reference):
  *   y[m, n] = sum_k a[m, k] * w[n, k] + bias[n], summed in fp32;  out = out_dtype(y),
- *   out_dtype(gelu_tanh(out_dtype(y))) with XGEN_ACT_GELU_TANH, or with a residual (BF16, no activation)
- *   bf16(residual[m] + bf16(bf16(y) * gate_table[indices[m % seq]])), the roundings of xgen_w8a8_gate_residual.
+ *   out_dtype(gelu_tanh(y)) with XGEN_ACT_GELU_TANH, or with a residual (BF16, no activation)
+ *   bf16(residual[m] + y * gate_table[indices[m % seq]]): one rounding each, where the 8-bit products' have two and three.
  * a [M, K], w [N, K]: codes and scales as xgen_mxfp4_quantize lays them out (lda, ldw and block strides in bytes).
  * A row or weight row with a scale of 255 gives NaN.  bias: NULL or [N] of BF16, F16 or F32.  residual NULL or BF16
  * [M, N]; gate_table BF16 [gate_rows, N] with indices int64 [seq], M a multiple of seq (an index outside: a NaN row).

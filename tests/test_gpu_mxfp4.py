@@ -380,3 +380,45 @@ def test_installed_in_a_model(cuda):
     assert isinstance(got[0], MXFP4Linear) and isinstance(got[2], MXFP4Linear)
     check_product(quantize_mxfp4(x, rounding="ceil"), w, 5, 96, 64, bias, got=got[0](x))
     assert got(x).shape == (5, 32)
+
+
+def rounded_once(cuda, g, m, n, k, form):
+    """The form's rows against 64 bits, within its sums' error and half a step."""
+    a, w = packed(g, m, k, spread=0), packed(g, n, k, 0.02, spread=0)
+    at = torch.cat([torch.arange(min(m, 40)), torch.randperm(m, generator=g)[:60], torch.arange(max(0, m - 40), m)]).unique()
+    part = (a[0][at.to(cuda)], pack_scales(unpack_scales(a[1], m, k)[at.to(cuda)]))
+    av, wv = values(part, len(at), k), values(w, n, k)
+    y, error = av @ wv.t(), -(-k // 64) * 2.0 ** -22 * (av.abs() @ wv.abs().t())
+    if form == "gated":
+        res, gate, idx = gated_inputs(g, cuda, m, n, 7, m)
+        got = mxfp4_matmul(*a, *w, residual=res, gate_table=gate, indices=idx)
+        t = gate.double().cpu()[idx.cpu()[at]]
+        want = res.double().cpu()[at] + y * t
+        error = error * t.abs() + 2.0 ** -24 * want.abs()
+    elif form == "plain":
+        got, want = mxfp4_matmul(*a, *w), y
+    else:
+        got, want = mxfp4_matmul(*a, *w, activation="gelu_tanh", out_dtype=form), gelu(y)
+        error = 1.13 * error + 2.0 ** -20 * y.abs() + 1e-30
+    f = torch.finfo(got.dtype)
+    error = error + f.eps / 2 * (want.abs() + error) + f.smallest_normal * f.eps
+    off = (got[at.to(cuda)].double().cpu() - want).abs() - error
+    assert bool((off <= 0).all()), (float(off.max()), divmod(int(off.argmax()), n))
+
+
+@pytest.mark.parametrize("form", ["gated", BF, HF])
+def test_one_rounding(cuda, form):
+    """A gated residual and GELU are formed from the sums in 32 bits, on every tile."""
+    g = torch.Generator().manual_seed(12)
+    for t, (m, n, k) in sorted(tile_shapes(form == "gated").items()):
+        print("tile", t, "of", (m, n, k), flush=True)
+        rounded_once(cuda, g, m, n, k, form)
+
+
+@pytest.mark.parametrize("form", ["gated", "plain", BF])
+@pytest.mark.parametrize("k", [32, 256, 288, 544, 800, 1312])
+def test_short_sums_of_many_tiles(cuda, k, form):
+    """One to six pairs of K on the large tiles, three tiles a workgroup: each tile's start lies among the one before's stores."""
+    m, n = 7900, 5392
+    assert tile(m, n, k, form == "gated") == (256, 256)
+    rounded_once(cuda, torch.Generator().manual_seed(k), m, n, k, form)

@@ -346,8 +346,29 @@ void gemm_tile_kernel(GemmArgs p) {
   const int half = lane >> 5;
   // acc[i][j] element e: feature n0 + wn*32*FN + i*32 + (e/4)*8 + (lane/32)*4 + e%4,
   //                      token   m0 + wm*32*FM + j*32 + lane%32
+  // MXFP4 with a gated residual rounds once: the residual's pieces lie in the tile's place, where the lane that rounds
+  // a value finds it, and the gate is read there (its rows are few, and cached)
+  constexpr bool kGatedHere = GATED && kMx;
+  [[maybe_unused]] uint32_t gate_row[FM];  // byte offset of a token's gate row, or kOutOfRange: an index outside the table
+  if constexpr (kGatedHere) {
+    const __amdgpu_buffer_rsrc_t rind = rsrc(p.indices, p.seq * 8);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t m = (uint32_t)(m0 + wm * 32 * FM + j * 32 + (lane & 31)), mq = (__umulhi(m, p.seq_magic) + m) >> p.seq_shift;
+      const u32x2 g = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rind, (m - mq * p.seq) * 8, 0, 0));
+      gate_row[j] = g.y == 0 && g.x < (uint32_t)p.gate_rows ? g.x * (uint32_t)p.gate_stride * 2 : kOutOfRange;
+    }
+    load_res(kResAhead, kSteps);
+#pragma unroll
+    for (int q = 0; q < kSteps; ++q) {
+      const int c = q * C::kThreads + tid;
+      *reinterpret_cast<u32x4 *>(smem + c / kChunks * C::kRowPitch + c % kChunks * 16) = res[q];
+    }
+    __syncthreads();
+  }
   auto round_tile = [&](auto OUT, auto ACT) {
     constexpr int kOut = decltype(OUT)::value, kAct = decltype(ACT)::value;
+    [[maybe_unused]] const __amdgpu_buffer_rsrc_t rgate = rsrc(p.gate, GATED ? p.gate_bytes : 0);
     float sam[FM];
 #pragma unroll
     for (int j = 0; j < FM; ++j) sam[j] = prm[wm * 32 * FM + j * 32 + (lane & 31)];
@@ -365,10 +386,22 @@ void gemm_tile_kernel(GemmArgs p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             y[e] = __builtin_fmaf(T::to_f32(acc[i][j][gq * 4 + e]), sam[j] * swr[e], bir[e]);
-            if constexpr (kAct == XGEN_ACT_GELU_TANH) y[e] = gelu_tanh(round_out<kOut>(y[e]));
+            if constexpr (kAct == XGEN_ACT_GELU_TANH) y[e] = gelu_tanh(kMx ? y[e] : round_out<kOut>(y[e]));
           }
-          *reinterpret_cast<u32x2 *>(smem + ml * C::kRowPitch + nl * 2) =
-              u32x2{pack_out<kOut>(y[0], y[1]), pack_out<kOut>(y[2], y[3])};
+          u32x2 *const at = reinterpret_cast<u32x2 *>(smem + ml * C::kRowPitch + nl * 2);
+          if constexpr (kGatedHere) {
+            const bool known = gate_row[j] != kOutOfRange;
+            const u32x2 t = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_raw_buffer_load_b64(rgate, known && n0 + nl < p.N ? gate_row[j] + (n0 + nl) * 2 : kOutOfRange, 0, 0));
+            const u32x2 r = *at;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int up = e & 1 ? 0 : 16;  // (the upper value's bits in place, the lower's shifted there)
+              const float te = __uint_as_float(t[e / 2] << up & 0xffff0000u), re = __uint_as_float(r[e / 2] << up & 0xffff0000u);
+              y[e] = known ? __builtin_fmaf(y[e], te, re) : __builtin_nanf("");
+            }
+          }
+          *at = u32x2{pack_out<kOut>(y[0], y[1]), pack_out<kOut>(y[2], y[3])};
           if (p.acc_out) {
             const int m = m0 + ml, n = n0 + nl;
             if (m < p.M && n < p.N) {
@@ -391,7 +424,7 @@ void gemm_tile_kernel(GemmArgs p) {
     if (p.act == XGEN_ACT_NONE) round_tile(F16(), NoAct());
     else round_tile(F16(), Gelu());
   }
-  if constexpr (GATED) load_res(kResAhead, kSteps);
+  if constexpr (GATED && !kMx) load_res(kResAhead, kSteps);
   __syncthreads();
 
   // rows of 16-byte pieces, consecutive lanes on consecutive pieces of a row; rows past M
@@ -411,10 +444,11 @@ void gemm_tile_kernel(GemmArgs p) {
           rgate, in && ok ? (g.x * (uint32_t)p.gate_stride + col) * 2 : kOutOfRange, 0, 0);
     }
   };
-  if constexpr (GATED) load_gate(0);
+  constexpr bool kGateRows = GATED && !kMx;
+  if constexpr (kGateRows) load_gate(0);
 #pragma unroll
   for (int q0 = 0; q0 < kSteps; q0 += kUnroll) {
-    if constexpr (GATED) {
+    if constexpr (kGateRows) {
       __builtin_amdgcn_sched_barrier(0);  // (a later group's reads stay behind this one's: registers)
       if (q0 + kUnroll < kSteps) load_gate(q0 + kUnroll);
     }
@@ -424,7 +458,7 @@ void gemm_tile_kernel(GemmArgs p) {
       uint32_t row, col;
       const bool in = piece(q0 + u, row, col);
       u32x4 v = *reinterpret_cast<const u32x4 *>(smem + c / kChunks * C::kRowPitch + c % kChunks * 16);
-      if constexpr (GATED) {
+      if constexpr (kGateRows) {
         const u32x2 g = gidx[q0 + u];
         v = g.y == 0 && g.x < (uint32_t)p.gate_rows
                 ? gate_residual8(res[q0 + u], v, gt[(q0 / kUnroll) & 1][u])

@@ -328,37 +328,59 @@ void mx4_gemm_kernel(GemmArgs p) {
     const int feature = wn * kWaveRows + (el >> 5) * 8;  // + i * 32 + m * 16
     const uint8_t *pb = smem + kBiasBase + (tile_i % kBiasSets) * kBiasBytes;
     uint8_t *xb = smem + kXposeBase + wave * kXpose;
-    uint8_t *xw = xb + (el & 31) * kXposeRow + (el >> 5) * 16;
-    const uint8_t *xr = xb + (el >> 3) * kXposeRow + (el & 7) * 16;
-    // this lane's pieces of what is read back: 8 features of rows + 8 q of each 32 tokens
-    const int col = n0 + wn * kWaveRows + (el & 7) * 8;                   // + h * 64
-    const uint32_t row = (uint32_t)(m0 + wm * kWaveRows + (el >> 3));     // + j * 32 + q * 8
-    const uint32_t at = (row * (uint32_t)p.ldo + (uint32_t)col) * 2;      // rows past M lie past the output's bytes
-    const uint32_t step8 = 16 * (uint32_t)p.ldo;                          // bytes of 8 rows
+    uint8_t *xw = xb + (el & 31) * kXposeRow + (el >> 5) * (GATED ? 32 : 16);
+    // this lane's pieces of what is read back: 8 features of kPieces rows of each 32 tokens, kBetween apart
+    constexpr int kLanes = GATED ? 4 : 8, kBetween = 64 / kLanes, kPieces = 32 / kBetween;
+    const uint8_t *xr = xb + el / kLanes * kXposeRow + el % kLanes * (GATED ? 32 : 16);
+    const int col = n0 + wn * kWaveRows + el % kLanes * 8;                   // + the block's first feature
+    const uint32_t row = (uint32_t)(m0 + wm * kWaveRows + el / kLanes);      // + j * 32 + q * kBetween
+    const uint32_t at = (row * (uint32_t)p.ldo + (uint32_t)col) * 2;         // rows past M lie past the output's bytes
+    const uint32_t step = kBetween * 2 * (uint32_t)p.ldo;                    // bytes of kBetween rows
     [[maybe_unused]] __amdgpu_buffer_rsrc_t rres, rgate;
-    [[maybe_unused]] uint32_t gate_row[F][4];  // byte offset, or kOutOfRange: an index outside the table
-    [[maybe_unused]] u32x4 res[4], gate[4];
+    [[maybe_unused]] uint32_t gate_row[F][kPieces];  // byte offset, or kOutOfRange: an index outside the table
+    [[maybe_unused]] u32x4 res[kPieces], gate[kPieces];
     if constexpr (GATED) {
       rres = rsrc(p.residual, p.residual_bytes);
       rgate = rsrc(p.gate, p.gate_bytes);
       const __amdgpu_buffer_rsrc_t rind = rsrc(p.indices, p.seq * 8);
 #pragma unroll
-      for (int n = 0; n < 4 * F; ++n) {
-        const uint32_t m = row + n * 8, mq = (__umulhi(m, p.seq_magic) + m) >> p.seq_shift;
+      for (int n = 0; n < kPieces * F; ++n) {
+        const uint32_t m = row + n * kBetween, mq = (__umulhi(m, p.seq_magic) + m) >> p.seq_shift;
         const u32x2 index = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rind, (m - mq * p.seq) * 8, 0, 0));
-        gate_row[n / 4][n % 4] = index.y == 0 && index.x < (uint32_t)p.gate_rows ? index.x * (uint32_t)p.gate_stride * 2 : kOutOfRange;
+        gate_row[n / kPieces][n % kPieces] = index.y == 0 && index.x < (uint32_t)p.gate_rows ? index.x * (uint32_t)p.gate_stride * 2 : kOutOfRange;
       }
     }
-    u32x4 pending[4];
-    auto store = [&](int h, int j) {
+    u32x4 pending[kPieces][GATED ? 2 : 1];  // as read back: rounded, or with a gated residual in fp32
+    auto store = [&](int first, int j) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        u32x4 v = pending[q];
-        if constexpr (GATED)
-          v = gate_row[j][q] != kOutOfRange ? gate_residual8(res[q], v, gate[q])
+      for (int q = 0; q < kPieces; ++q) {
+        u32x4 v = pending[q][0];
+        if constexpr (GATED) {
+          const f32x4 lo = __builtin_bit_cast(f32x4, pending[q][0]), hi = __builtin_bit_cast(f32x4, pending[q][1]);
+          const float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          v = gate_row[j][q] != kOutOfRange ? gate_residual8(res[q], y, gate[q])
                                             : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-        __builtin_amdgcn_raw_buffer_store_b128(v, ro, col + h * 64 < p.N ? at + (j * 4 + q) * step8 + h * 128 : kOutOfRange, 0,
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(v, ro, col + first < p.N ? at + (j * kPieces + q) * step + first * 2 : kOutOfRange, 0,
                                                kCachePolicyNT);
+      }
+    };
+    // what has passed the transpose area: 32 tokens (j) of the features from `first` on; the step before is stored while
+    // this one's rows are read back (a wave's LDS operations complete in order)
+    auto read_back = [&](int first, int j) {
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q) {
+        const u32x4 *from = reinterpret_cast<const u32x4 *>(xr + q * kBetween * kXposeRow);
+        pending[q][0] = from[0];
+        if constexpr (GATED) {
+          pending[q][1] = from[1];
+          const uint32_t c = (uint32_t)(col + first);
+          const bool in = c < (uint32_t)p.N;
+          res[q] = __builtin_amdgcn_raw_buffer_load_b128(
+              rres, in ? ((row + j * 32 + q * kBetween) * (uint32_t)p.ld_residual + c) * 2 : kOutOfRange, 0, 0);
+          gate[q] = __builtin_amdgcn_raw_buffer_load_b128(
+              rgate, in && gate_row[j][q] != kOutOfRange ? gate_row[j][q] + c * 2 : kOutOfRange, 0, 0);
+        }
       }
     };
     float bias[2][16];
@@ -377,31 +399,28 @@ void mx4_gemm_kernel(GemmArgs p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         y[e] += bias[ii][e];
-        if constexpr (ACT == XGEN_ACT_GELU_TANH) y[e] = gelu_tanh(round_out<OUT_DT>(y[e]));
+        if constexpr (ACT == XGEN_ACT_GELU_TANH) y[e] = gelu_tanh(y[e]);
       }
+      if constexpr (GATED) {
+        // in fp32, a fragment's 32 features at a time: the product with the gate and the sum are rounded once
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-        *reinterpret_cast<u32x4 *>(xw + ii * 64 + m * 32) =
-            u32x4{pack_out<OUT_DT>(y[8 * m], y[8 * m + 1]), pack_out<OUT_DT>(y[8 * m + 2], y[8 * m + 3]),
-                  pack_out<OUT_DT>(y[8 * m + 4], y[8 * m + 5]), pack_out<OUT_DT>(y[8 * m + 6], y[8 * m + 7])};
-      if constexpr (ii == 1) {
-        // the step before is stored while this one's rows are read back (a wave's LDS operations complete in order)
-        if constexpr (n > 1) store((n - 2) / 8, (n - 2) / 2 % 4);
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<f32x4 *>(xw + e / 8 * 64 + e % 8 * 4) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        if constexpr (n > 0) store(((n - 1) / 8 * 2 + (n - 1) % 2) * 32, (n - 1) / 2 % 4);
+        read_back(i * 32, j);
+      } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          pending[q] = *reinterpret_cast<const u32x4 *>(xr + q * 8 * kXposeRow);
-          if constexpr (GATED) {
-            const uint32_t c = (uint32_t)(col + h * 64);
-            const bool in = c < (uint32_t)p.N;
-            res[q] = __builtin_amdgcn_raw_buffer_load_b128(
-                rres, in ? ((row + j * 32 + q * 8) * (uint32_t)p.ld_residual + c) * 2 : kOutOfRange, 0, 0);
-            gate[q] = __builtin_amdgcn_raw_buffer_load_b128(
-                rgate, in && gate_row[j][q] != kOutOfRange ? gate_row[j][q] + c * 2 : kOutOfRange, 0, 0);
-          }
+        for (int m = 0; m < 2; ++m)
+          *reinterpret_cast<u32x4 *>(xw + ii * 64 + m * 32) =
+              u32x4{pack_out<OUT_DT>(y[8 * m], y[8 * m + 1]), pack_out<OUT_DT>(y[8 * m + 2], y[8 * m + 3]),
+                    pack_out<OUT_DT>(y[8 * m + 4], y[8 * m + 5]), pack_out<OUT_DT>(y[8 * m + 6], y[8 * m + 7])};
+        if constexpr (ii == 1) {
+          if constexpr (n > 1) store((n - 2) / 8 * 64, (n - 2) / 2 % 4);
+          read_back(h * 64, j);
         }
       }
     });
-    store(1, F - 1);
+    store(GATED ? (F - 1) * 32 : 64, F - 1);
     mma<acc_reg(F - 1, F - 1), 1, false>(wf[0][1][F - 1], xf[0][1][F - 1], sc[0][F - 1], sc[0][2 * F - 1]);
     // the rest of a stage A, for the next tile's first pair (behind the epilogue, which needs the fragments' registers)
 #pragma unroll

@@ -160,6 +160,16 @@ __device__ __forceinline__ u32x4 gate_residual8(const u32x4 &r, const u32x4 &y, 
   return u32x4{o[0], o[1], o[2], o[3]};
 }
 
+// Eight values of bf16(r + y t), y in fp32: one rounding.
+__device__ __forceinline__ u32x4 gate_residual8(const u32x4 &r, const float (&y)[8], const u32x4 &t) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    o[i] = pack_bf16x2(__builtin_fmaf(y[2 * i], __uint_as_float(t[i] << 16), __uint_as_float(r[i] << 16)),
+                       __builtin_fmaf(y[2 * i + 1], __uint_as_float(t[i] & 0xffff0000u), __uint_as_float(r[i] & 0xffff0000u)));
+  return o;
+}
+
 // --- OCP e4m3fn packing -----------------------------------------------------
 // v_cvt_pk_fp8_f32 rounds to nearest even into e4m3fn (gfx950: OCP format).
 // Inputs here are always finite and within [-448, 448].

@@ -83,8 +83,8 @@ def mxfp4_matmul(codes, scales, weight, weight_scales, *, bias=None, out_dtype=t
                  residual=None, gate_table=None, indices=None):
     """[..., N]: rows of packed activations [..., K/2] times packed weights [N, K/2], each with its scales, summed in fp32,
     plus bias [N] (BF16/F16/F32); its GELU-tanh with activation "gelu_tanh".  With residual BF16 of the output's
-    shape, gate_table BF16 [T, N] and indices int64 [S]: residual + gate_table[indices[position]] * that, rounded
-    as H3FP8Linear.forward_gate_residual's (S: the rows' last leading dimension, or a divisor of the rows)."""
+    shape, gate_table BF16 [T, N] and indices int64 [S]: residual + gate_table[indices[position]] * that
+    (S: the rows' last leading dimension, or a divisor of the rows).  Every form is rounded once, from fp32."""
     _inference_only(bias, residual, gate_table)
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unsupported activation {activation!r}")
