@@ -572,8 +572,8 @@ int xgen_mxfp4_dequantize(const void *codes, int64_t ld_codes, const void *scale
  *   y[m, n] = sum_k a[m, k] * w[n, k] + bias[n], summed in fp32;  out = out_dtype(y),
  *   out_dtype(gelu_tanh(y)) with XGEN_ACT_GELU_TANH, or with a residual (BF16, no activation)
  *   bf16(residual[m] + y * gate_table[indices[m % seq]]): one rounding each, where the 8-bit products' have two and three.
- * a [M, K], w [N, K]: codes and scales as xgen_mxfp4_quantize lays them out (lda, ldw and block strides in bytes).
- * A row or weight row with a scale of 255 gives NaN.  bias: NULL or [N] of BF16, F16 or F32.  residual NULL or BF16
+ * a [M, K], w [N, K]: codes and scales as xgen_mxfp4_quantize lays them out (lda, ldw and block strides in bytes), zeros
+ * for the blocks past K included.  A row or weight row with a scale of 255 gives NaN.  bias: NULL or [N] of BF16, F16 or F32.  residual NULL or BF16
  * [M, N]; gate_table BF16 [gate_rows, N] with indices int64 [seq], M a multiple of seq (an index outside: a NaN row).
  * K a multiple of 32, N of 16; rows, bias and scale blocks 16-byte aligned; w below 2 GiB.  out overlaps no operand.
  */

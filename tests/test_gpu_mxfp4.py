@@ -422,3 +422,22 @@ def test_short_sums_of_many_tiles(cuda, k, form):
     m, n = 7900, 5392
     assert tile(m, n, k, form == "gated") == (256, 256)
     rounded_once(cuda, torch.Generator().manual_seed(k), m, n, k, form)
+
+
+def test_gated_chunks_of_odd_rows(cuda):
+    """An output above 2 GiB whose chunks are whole sequences of odd length: the second one starts at an odd row of the scales
+    and ends with them."""
+    seq, n, k = 33025, 16384, 64
+    m = 2 * seq
+    g = torch.Generator(device=cuda).manual_seed(13)
+    sa = torch.randint(120, 130, (m, k // 32), generator=g, device=cuda, dtype=U8)
+    a = (torch.randint(0, 256, (m, k // 2), generator=g, device=cuda, dtype=U8), pack_scales(sa))
+    w = (torch.randint(0, 256, (n, k // 2), generator=g, device=cuda, dtype=U8), pack_scales(torch.randint(120, 130, (n, k // 32), generator=g, device=cuda, dtype=U8)))
+    res = torch.randn((m, n), generator=g, device=cuda, dtype=BF)
+    gate = torch.randn((5, n), generator=g, device=cuda, dtype=BF)
+    idx = torch.randint(0, 5, (seq,), generator=g, device=cuda)
+    out = mxfp4_matmul(*a, *w, residual=res, gate_table=gate, indices=idx)
+    for first, last in ((0, 40), (seq - 60, seq + 61), (m - 300, m), (m - 41, m), (m - 1, m)):
+        at = torch.arange(first, last, device=cuda) % seq
+        part = mxfp4_matmul(a[0][first:last], pack_scales(sa[first:last]), *w, residual=res[first:last], gate_table=gate, indices=idx[at])
+        assert torch.equal(out[first:last], part), first

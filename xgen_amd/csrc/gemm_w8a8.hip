@@ -610,6 +610,7 @@ struct GateParams {  // the gated residual epilogue's inputs (null residual: pla
 struct BlockScales {  // the MXFP4 kind's scale bytes (xgen_mxfp4_quantize's layout) in place of sa and sw
   const uint8_t *x = nullptr;
   int64_t x_block = 0;  // bytes between the blocks of 256 values
+  int64_t x_rows = 0;   // rows of a block from x on: a multiple of two for the whole call, not for each chunk of it
   const uint8_t *w = nullptr;
   int64_t w_block = 0;
 };
@@ -678,7 +679,7 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
       GateParams gc = gp;
       if (gated) gc.residual = static_cast<const uint8_t *>(gp.residual) + m0 * gp.ld_residual * 2;
       BlockScales bc = bs;
-      if (kMx) bc.x = bs.x + m0 * 8;
+      if (kMx) bc.x = bs.x + m0 * 8, bc.x_rows = bs.x_rows - m0;
       const int st = gemm_entry<KIND>(
           fn, static_cast<const uint8_t *>(a) + m0 * lda, lda, w, ldw, mi, N, K, sa_stride ? sa + m0 : sa, sa_stride,
           sw, sw_stride, bias, bias_dtype, activation, static_cast<uint8_t *>(out) + m0 * ldo * 2, out_dtype, ldo,
@@ -743,7 +744,8 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   g.ws = bs.w;
   g.xs_block = bs.x_block;
   g.ws_block = bs.w_block;
-  g.xs_rows = (uint32_t)((M + M % 2) * 8);  // (below 2^31: M rows of at least 16 bytes are)
+  // (below 2^31: M rows of at least 16 bytes are; a last chunk that starts at an odd row has no row behind its own)
+  g.xs_rows = (uint32_t)((M % 2 && M < bs.x_rows ? M + 1 : M) * 8);
   g.ws_rows = (uint32_t)(N * 8);
   g.kt4 = (int)(((K + BK - 1) / BK + 3) / 4 * 4);
   const int64_t out_bytes = ((M - 1) * ldo + N) * 2;
@@ -867,6 +869,7 @@ extern "C" int xgen_mxfp4_matmul(const void *a, int64_t lda, const void *a_scale
   BlockScales bs;
   bs.x = static_cast<const uint8_t *>(a_scales);
   bs.x_block = a_block_stride;
+  bs.x_rows = M + M % 2;
   bs.w = static_cast<const uint8_t *>(w_scales);
   bs.w_block = w_block_stride;
   return gemm_entry<kMx4>(fn, a, lda, w, ldw, M, N, K / 2, nullptr, 0, nullptr, 0, bias, bias_dtype, activation, out,

@@ -18,10 +18,10 @@
 // 128-byte line (stored from the accumulators' places, 32 bytes of a row at a time, the epilogue took 142 us of
 // the call below).  Past the caches: the output is more than they hold wherever this kernel's tiles fill the card.
 //
-// What bounds it: the matrix units' power.  15,624 x 14,336 x 5,376 takes 550 us, 4.4 PFLOP/s: 1.69 us a pair and CU on
-// normally distributed values, 1.02 on zeros, with the same instructions; a loop of these MFMAs alone does 6.2 to
-// 6.7 PFLOP/s on random codes, 9.65 on zeros.  GELU adds 42 us (its arithmetic stands between the MFMAs of an epilogue),
-// the gated residual 70.
+// What bounds it: the matrix units' power.  15,624 x 14,336 x 5,376 takes 532 to 550 us, 4.4 PFLOP/s: 1.69 us a pair and CU
+// on normally distributed values, 1.02 on zeros, with the same instructions; a loop of these MFMAs alone does 6.2 to
+// 6.7 PFLOP/s on random codes, 9.65 on zeros.  GELU there 582 to 600 (its arithmetic stands between the MFMAs of an epilogue).
+// 15,624 x 5,376 x 14,336: 553 us, GELU 570, the gated residual 634 (its reads are waited for).
 //
 // The same on the fragments of 16 x 16 x 128, which draw less power (7.3 PFLOP/s in the loop): 575 us; there are twice
 // as many MFMAs and reads of scales to issue, and the power saved is not what it gained.

@@ -81,7 +81,8 @@ def unpack_scales(scales, rows, K):
 
 def mxfp4_matmul(codes, scales, weight, weight_scales, *, bias=None, out_dtype=torch.bfloat16, activation=None,
                  residual=None, gate_table=None, indices=None):
-    """[..., N]: rows of packed activations [..., K/2] times packed weights [N, K/2], each with its scales, summed in fp32,
+    """[..., N]: rows of packed activations [..., K/2] times packed weights [N, K/2], each with its scales
+    (quantize_mxfp4's or pack_scales', zeros in the padding), summed in fp32,
     plus bias [N] (BF16/F16/F32); its GELU-tanh with activation "gelu_tanh".  With residual BF16 of the output's
     shape, gate_table BF16 [T, N] and indices int64 [S]: residual + gate_table[indices[position]] * that
     (S: the rows' last leading dimension, or a divisor of the rows).  Every form is rounded once, from fp32."""
@@ -151,7 +152,7 @@ class MXFP4Linear(nn.Module):
                             activation=self.activation)
 
     def forward_gate_residual(self, x, residual, gate_table, indices):
-        """`residual + bf16(gate_table[indices] * self(x))` with the gated residual in the product's epilogue.
+        """`residual + gate_table[indices] * self(x)`, rounded once, in the product's epilogue.
         x BF16/F16 [B, S, K]; residual BF16 [B, S, N]; gate_table BF16 [T, N]; indices int64 [S]."""
         if self.activation not in (None, "none"):
             raise ValueError("forward_gate_residual needs no activation")
