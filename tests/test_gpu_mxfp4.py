@@ -441,3 +441,45 @@ def test_gated_chunks_of_odd_rows(cuda):
         at = torch.arange(first, last, device=cuda) % seq
         part = mxfp4_matmul(a[0][first:last], pack_scales(sa[first:last]), *w, residual=res[first:last], gate_table=gate, indices=idx[at])
         assert torch.equal(out[first:last], part), first
+
+
+def split(m, n, k, gated):
+    fn = ctypes.CDLL(str(N.library_path())).xgen_gemm_split_choice
+    fn.restype, fn.argtypes = ctypes.c_int64, [ctypes.c_int64] * 3 + [ctypes.c_int]
+    return fn(m, n, k // 2, int(gated))
+
+
+@pytest.mark.parametrize("form", ["gated", "plain", BF])
+def test_two_launches(cuda, form):
+    """Rows in two launches, an odd number of them: against 64 bits, and the bits of the last rows alone."""
+    m, n, k = 3911, 5376, 7200
+    first = split(m, n, k, form == "gated")
+    assert 0 < first < m and first % 256 == 0
+    g = torch.Generator().manual_seed(14)
+    rounded_once(cuda, g, m, n, k, form)
+    a, w = packed(g, m, k, spread=0), packed(g, n, k, 0.02, spread=0)
+    more, part_more = {}, {}
+    if form == "gated":
+        res, gate, _ = gated_inputs(g, cuda, m, n, 7, 1)
+        idx = torch.randint(0, 7, (m,), generator=g).to(cuda)
+        more = {"residual": res, "gate_table": gate, "indices": idx}
+        part_more = {"residual": res[first - 100:], "gate_table": gate, "indices": idx[first - 100:]}
+    elif form is BF:
+        more = part_more = {"activation": "gelu_tanh"}
+    part = mxfp4_matmul(a[0][first - 100:], pack_scales(unpack_scales(a[1], m, k)[first - 100:]), *w, **part_more)
+    assert torch.equal(mxfp4_matmul(*a, *w, **more)[first - 100:], part)
+
+
+def test_two_launches_of_sequences(cuda):
+    """Seven sequences of 559 rows: the second launch's first row is no sequence's first."""
+    seq, n, k = 559, 5376, 7200
+    m = 7 * seq
+    first = split(m, n, k, True)
+    assert first and first % seq
+    g = torch.Generator().manual_seed(15)
+    a, w = packed(g, m, k, spread=0), packed(g, n, k, 0.02, spread=0)
+    res, gate, idx = gated_inputs(g, cuda, m, n, 7, seq)
+    whole = mxfp4_matmul(*a, *w, residual=res, gate_table=gate, indices=idx)
+    want = mxfp4_matmul(*a, *w, residual=res, gate_table=gate, indices=idx.repeat(7))
+    assert torch.equal(whole, want)
+    check_gated(a, w, m, n, k, None, res, gate, idx, whole)

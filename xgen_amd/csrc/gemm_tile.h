@@ -354,7 +354,7 @@ void gemm_tile_kernel(GemmArgs p) {
     const __amdgpu_buffer_rsrc_t rind = rsrc(p.indices, p.seq * 8);
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const uint32_t m = (uint32_t)(m0 + wm * 32 * FM + j * 32 + (lane & 31)), mq = (__umulhi(m, p.seq_magic) + m) >> p.seq_shift;
+      const uint32_t m = (uint32_t)(m0 + wm * 32 * FM + j * 32 + (lane & 31)) + p.seq_first, mq = (__umulhi(m, p.seq_magic) + m) >> p.seq_shift;
       const u32x2 g = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rind, (m - mq * p.seq) * 8, 0, 0));
       gate_row[j] = g.y == 0 && g.x < (uint32_t)p.gate_rows ? g.x * (uint32_t)p.gate_stride * 2 : kOutOfRange;
     }

@@ -123,6 +123,21 @@ int choose_gemm_tile(int kind, int64_t M, int64_t N, int64_t K, bool gated, bool
   return best;
 }
 
+// An output of little more than whole rounds of 256 x 256 tiles leaves most CUs idle in its last one: the tile-rows of whole
+// rounds are then a launch, and the rows behind them another on the tile that suits them.  (Splitting the last tiles' K
+// instead would make a row's sum depend on the rows beside it.)  5% at least, as the sums put it, with 3 us for the launch:
+// 3,906 x 5,376 x 14,336 160 us, as one launch 182; 15,624 rows of it 530 and 566; 4,400 x 4,096 x 4,096 45 and 56.
+int64_t split_mx4_rows(int64_t M, int64_t N, int64_t K, bool gated) {
+  const int64_t tiles_n = (N + kTileN - 1) / kTileN, cus = device_cu_count();
+  const int64_t first = (M + kTileM - 1) / kTileM * tiles_n / cus * cus / tiles_n * kTileM;
+  if (first <= 0 || first >= M) return 0;
+  auto cost = [&](int64_t rows) {
+    const int t = choose_gemm_tile(kMx4, rows, N, K, gated, false);
+    return tile_cost(kMx4, t < 0 ? kTiles : t, rows, N, K);
+  };
+  return cost(first) + cost(M - first) + 3.0f < 0.95f * cost(M) ? first : 0;
+}
+
 void launch_gemm_tile(int kind, int tile, const GemmArgs &g, hipStream_t stream) {
   if (kind == kInt8) launch_kind<kInt8>(tile, g, stream);
   else if (kind == kFp8) launch_kind<kFp8>(tile, g, stream);
@@ -139,4 +154,9 @@ extern "C" int xgen_gemm_tile_choice(int kind, int64_t M, int64_t N, int64_t K, 
   const xgen::TileSize t = xgen::kTileSizes[tile < 0 ? xgen::kTiles : tile];
   *n = t.n;
   return t.m;
+}
+
+// The same for a call's rows in its first launch, 0 where it is one launch.
+extern "C" int64_t xgen_gemm_split_choice(int64_t M, int64_t N, int64_t K, int gated) {
+  return xgen::split_mx4_rows(M, N, K, gated != 0);
 }

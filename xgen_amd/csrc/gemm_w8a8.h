@@ -40,6 +40,7 @@ struct GemmArgs {
   int64_t gate_rows;
   const int64_t *indices;
   uint32_t seq, seq_magic, seq_shift;  // m % seq = m - ((mulhi(m, magic) + m) >> shift) * seq
+  uint32_t seq_first;  // MXFP4: row 0's place in its sequence
   uint32_t residual_bytes, gate_bytes;  // (M - 1) * ld_residual * 2 + N * 2, (gate_rows - 1) * gate_stride * 2 + N * 2
   // scale bytes of 32 values (kMx4 only): 8 bytes per row and 256 values, xs_block / ws_block bytes between two
   // such blocks of all rows; bytes of one block's rows (an even number of them)
@@ -64,6 +65,8 @@ enum Kind { kInt8 = 0, kFp8 = 1, kFp8Exact = 2, kMx4 = 3 };  // (K, lda and ldw 
 
 // The smaller tile that a call runs on, or -1: the 256 x 256 kernel (gemm_tile.hip).
 int choose_gemm_tile(int kind, int64_t M, int64_t N, int64_t K, bool gated, bool accumulators);
+// Rows of an MXFP4 call's first launch, where two take less time than one: 0 for one.
+int64_t split_mx4_rows(int64_t M, int64_t N, int64_t K, bool gated);
 // Launches the call on that tile.  g: filled as for the 256 x 256 kernel.
 void launch_gemm_tile(int kind, int tile, const GemmArgs &g, hipStream_t stream);
 

@@ -732,7 +732,7 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   g.gate_rows = gp.gate_rows;
   g.indices = gp.indices;
   g.seq = (uint32_t)gp.seq;
-  g.seq_magic = g.seq_shift = 0;  // (read by the gated kernels only)
+  g.seq_magic = g.seq_shift = g.seq_first = 0;  // (read by the gated kernels only)
   if (gated) {
     const FastDiv fd = make_fastdiv((uint32_t)gp.seq);
     g.seq_magic = fd.m;
@@ -757,25 +757,58 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   g.out_bytes = (uint32_t)out_bytes;
   g.act = activation;
   g.out_dtype = out_dtype;
-  const int tile = choose_gemm_tile(KIND, M, N, K, gated, acc_out != nullptr);
-  if (tile >= 0) {
-    launch_gemm_tile(KIND, tile, g, stream);
+  if constexpr (kMx) {
+    auto run = [&](const GemmArgs &r) {
+      const int t = choose_gemm_tile(kMx4, r.M, N, K, gated, false);
+      if (t >= 0) launch_gemm_tile(kMx4, t, r, stream);
+      else launch_mx4_gemm(r, stream);
+    };
+    // rows from m0 on (a multiple of 256) as a launch of their own
+    auto part = [&](int64_t m0, int64_t m) {
+      GemmArgs r = g;
+      r.M = (int)m;
+      r.tiles_m = (int)((m + kTileM - 1) / kTileM);
+      r.per_xcd = (r.tiles_m * r.tiles_n + 7) / 8;
+      r.a += m0 * lda;
+      r.a_bytes = (uint32_t)((m - 1) * lda + K);
+      r.xs += m0 * 8;
+      r.xs_rows = (uint32_t)((m % 2 && m0 + m < bs.x_rows ? m + 1 : m) * 8);
+      r.out = static_cast<uint8_t *>(out) + m0 * ldo * 2;
+      r.out_bytes = (uint32_t)(((m - 1) * ldo + N) * 2);
+      if (gated) {
+        r.residual += m0 * gp.ld_residual * 2;
+        r.residual_bytes = (uint32_t)(((m - 1) * gp.ld_residual + N) * 2);
+        r.seq_first = (uint32_t)(m0 % gp.seq);
+      }
+      return r;
+    };
+    const int64_t first = split_mx4_rows(M, N, K, gated);
+    if (first) {
+      run(part(0, first));
+      run(part(first, M - first));
+    } else {
+      run(g);
+    }
+    return launch_status(fn);
+  } else {
+    const int tile = choose_gemm_tile(KIND, M, N, K, gated, acc_out != nullptr);
+    if (tile >= 0) {
+      launch_gemm_tile(KIND, tile, g, stream);
+      return launch_status(fn);
+    }
+    const bool with_acc = acc_out != nullptr;
+    if (gated) {
+      // (the gated entry takes the FP8 and INT8 kinds only: no exact-kind instance)
+      if constexpr (KIND != kFp8Exact) launch_gemm_w4_gated<KIND>(g, stream);
+    } else if (activation == XGEN_ACT_NONE) {
+      if (out_dtype == XGEN_DTYPE_BF16) launch_gemm_w4<KIND, XGEN_ACT_NONE, XGEN_DTYPE_BF16>(g, with_acc, stream);
+      else launch_gemm_w4<KIND, XGEN_ACT_NONE, XGEN_DTYPE_F16>(g, with_acc, stream);
+    } else {
+      if (out_dtype == XGEN_DTYPE_BF16) launch_gemm_w4<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_BF16>(g, with_acc, stream);
+      else launch_gemm_w4<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_F16>(g, with_acc, stream);
+    }
     return launch_status(fn);
   }
-  const bool with_acc = acc_out != nullptr;
-  if constexpr (kMx) {
-    launch_mx4_gemm(g, stream);
-  } else if (gated) {
-    // (the gated entry takes the FP8 and INT8 kinds only: no exact-kind instance)
-    if constexpr (KIND != kFp8Exact) launch_gemm_w4_gated<KIND>(g, stream);
-  } else if (activation == XGEN_ACT_NONE) {
-    if (out_dtype == XGEN_DTYPE_BF16) launch_gemm_w4<KIND, XGEN_ACT_NONE, XGEN_DTYPE_BF16>(g, with_acc, stream);
-    else launch_gemm_w4<KIND, XGEN_ACT_NONE, XGEN_DTYPE_F16>(g, with_acc, stream);
-  } else {
-    if (out_dtype == XGEN_DTYPE_BF16) launch_gemm_w4<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_BF16>(g, with_acc, stream);
-    else launch_gemm_w4<KIND, XGEN_ACT_GELU_TANH, XGEN_DTYPE_F16>(g, with_acc, stream);
-  }
-  return launch_status(fn);
 }
 
 }  // namespace

@@ -21,7 +21,8 @@
 // What bounds it: the matrix units' power.  15,624 x 14,336 x 5,376 takes 532 to 550 us, 4.4 PFLOP/s: 1.69 us a pair and CU
 // on normally distributed values, 1.02 on zeros, with the same instructions; a loop of these MFMAs alone does 6.2 to
 // 6.7 PFLOP/s on random codes, 9.65 on zeros.  GELU there 582 to 600 (its arithmetic stands between the MFMAs of an epilogue).
-// 15,624 x 5,376 x 14,336: 553 us, GELU 570, the gated residual 634 (its reads are waited for).
+// 15,360 x 5,376 x 14,336 and 264 rows more in a launch of their own: 530 us, with the gated residual 587 (its reads are
+// waited for).
 //
 // The same on the fragments of 16 x 16 x 128, which draw less power (7.3 PFLOP/s in the loop): 575 us; there are twice
 // as many MFMAs and reads of scales to issue, and the power saved is not what it gained.
@@ -345,7 +346,7 @@ void mx4_gemm_kernel(GemmArgs p) {
       const __amdgpu_buffer_rsrc_t rind = rsrc(p.indices, p.seq * 8);
 #pragma unroll
       for (int n = 0; n < kPieces * F; ++n) {
-        const uint32_t m = row + n * kBetween, mq = (__umulhi(m, p.seq_magic) + m) >> p.seq_shift;
+        const uint32_t m = row + n * kBetween + p.seq_first, mq = (__umulhi(m, p.seq_magic) + m) >> p.seq_shift;
         const u32x2 index = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rind, (m - mq * p.seq) * 8, 0, 0));
         gate_row[n / kPieces][n % kPieces] = index.y == 0 && index.x < (uint32_t)p.gate_rows ? index.x * (uint32_t)p.gate_stride * 2 : kOutOfRange;
       }
