@@ -120,7 +120,7 @@ def enable_weight_quant_linear(model: nn.Module, quant_config: QuantLayerConfig,
     was released are skipped; LoRA '.base_layer' suffixes are undone in the
     replacement name.  dtype 'w8a8' (the reference's transformer path builds the
     W8A8 module for every CLI value, matmul.py:183) or 'mxfp4': MXFP4Linear modules,
-    4-bit weights and activations.
+    4-bit weights and activations, which take float32 inputs as BF16 too.
     """
     if dtype not in ('w8a8', 'mxfp4'):
         raise ValueError("xgen_amd provides 'w8a8' and 'mxfp4' modules")
@@ -133,7 +133,9 @@ def enable_weight_quant_linear(model: nn.Module, quant_config: QuantLayerConfig,
         bias = layer.bias.data if getattr(layer, 'bias', None) is not None else None
         if dtype == 'mxfp4':
             weight = layer.weight.data
-            quant_module = MXFP4Linear(weight.to(torch.bfloat16) if weight.dtype == torch.float32 else weight, bias)
+            # (float32 weights and activations are taken as BF16, as WeightQuantLinearModule takes them)
+            quant_module = MXFP4Linear(weight.to(torch.bfloat16) if weight.dtype == torch.float32 else weight, bias,
+                                       cast_float32=True)
         else:
             quant_module = WeightQuantLinearModule(layer.weight.data, bias, clean_name)
         if '.' in clean_name:

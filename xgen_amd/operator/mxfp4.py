@@ -105,16 +105,19 @@ def mxfp4_matmul(codes, scales, weight, weight_scales, *, bias=None, out_dtype=t
 class MXFP4Linear(nn.Module):
     """A projection in 4 bits: weights packed once (on the device they came from), activations quantized per call.
     weight BF16/F16 [N, K], N a multiple of 16, K of 32.  `weight_rounding` and `rounding` choose the scales of
-    weights and activations, `activation` "gelu_tanh" the epilogue."""
+    weights and activations, `activation` "gelu_tanh" the epilogue.  With `cast_float32` a float32 input is taken as BF16,
+    as WeightQuantLinearModule takes it (refused without)."""
 
-    def __init__(self, weight, bias=None, *, activation=None, weight_rounding="ceil", rounding="ceil"):
+    cast_float32 = False
+
+    def __init__(self, weight, bias=None, *, activation=None, weight_rounding="ceil", rounding="ceil", cast_float32=False):
         super().__init__()
         if weight.ndim != 2 or weight.shape[0] % 16 or weight.shape[1] % 32:
             raise ValueError("MXFP4Linear requires [N, K] with N a multiple of 16 and K of 32")
         packed, scales = quantize_mxfp4(_device_weight(weight), rounding=weight_rounding)
-        self._keep(packed.to(weight.device), scales.to(weight.device), bias, activation, rounding)
+        self._keep(packed.to(weight.device), scales.to(weight.device), bias, activation, rounding, cast_float32)
 
-    def _keep(self, packed, scales, bias, activation, rounding):
+    def _keep(self, packed, scales, bias, activation, rounding, cast_float32):
         if activation not in _ACTIVATIONS:
             raise ValueError(f"unsupported activation {activation!r}")
         _rounding(rounding)
@@ -124,10 +127,10 @@ class MXFP4Linear(nn.Module):
         self.register_buffer("weight", packed)
         self.register_buffer("weight_scales", scales)
         self.register_buffer("bias", bias.detach().clone() if bias is not None else None)
-        self.activation, self.rounding = activation, rounding
+        self.activation, self.rounding, self.cast_float32 = activation, rounding, bool(cast_float32)
 
     @classmethod
-    def from_packed(cls, weight, scales, bias=None, *, activation=None, rounding="ceil"):
+    def from_packed(cls, weight, scales, bias=None, *, activation=None, rounding="ceil", cast_float32=False):
         """Weights packed elsewhere: codes uint8 [N, K/2] and scale bytes [N, K/32], kept as they are."""
         if weight.dtype != torch.uint8 or weight.ndim != 2 or weight.shape[0] % 16 or weight.shape[1] % 16:
             raise ValueError("MXFP4Linear.from_packed requires uint8 codes [N, K/2] with N a multiple of 16 and K of 32")
@@ -135,13 +138,17 @@ class MXFP4Linear(nn.Module):
             raise ValueError("MXFP4Linear.from_packed requires one scale byte per 32 values, [N, K/32]")
         result = cls.__new__(cls)
         nn.Module.__init__(result)
-        result._keep(weight.contiguous(), pack_scales(scales), bias, activation, rounding)
+        result._keep(weight.contiguous(), pack_scales(scales), bias, activation, rounding, cast_float32)
         return result
 
+    def _cast(self, x):
+        return x.to(torch.bfloat16) if self.cast_float32 and x.dtype == torch.float32 else x
+
     def quantize_input(self, x):
-        return quantize_mxfp4(x, rounding=self.rounding)
+        return quantize_mxfp4(self._cast(x), rounding=self.rounding)
 
     def forward(self, x):
+        x = self._cast(x)
         if x.dtype not in (torch.bfloat16, torch.float16) or x.shape[-1] != self.in_features:
             raise ValueError(f"MXFP4Linear requires a BF16/FP16 [..., {self.in_features}] input")
         return self.forward_quantized(*self.quantize_input(x), out_dtype=x.dtype)
