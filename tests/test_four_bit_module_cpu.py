@@ -1,8 +1,10 @@
 """MXFP4Linear and its installer without a GPU: which inputs an installed module takes, and what the installer refuses."""
 import pytest
 import torch
+from torch import nn
 
-from xgen_amd.operator import mxfp4
+from xgen_amd.config import QuantLayerConfig
+from xgen_amd.operator import matmul, mxfp4
 
 BF, HF, F32, U8, I64 = torch.bfloat16, torch.float16, torch.float32, torch.uint8, torch.int64
 
@@ -25,3 +27,21 @@ def test_float32_inputs_are_cast_where_asked_for():
         linear(x.double())
     with pytest.raises(ValueError, match="input"):
         module()(x)
+
+
+@pytest.mark.parametrize("last", [nn.Linear(96, 24), nn.Linear(48, 32), nn.Linear(96, 32, dtype=torch.float64)])
+def test_installer_refuses_before_it_replaces(last):
+    """A layer without a 4-bit form: named, and the layers before it are as they were."""
+    model = nn.Sequential(nn.Linear(64, 96), nn.Sequential(nn.GELU(), last))
+    with pytest.raises(ValueError, match=r"exclude.*: 1\.1 \("):
+        matmul.enable_weight_quant_linear(model, QuantLayerConfig(), dtype="mxfp4")
+    assert type(model[0]) is nn.Linear and model[1][1] is last
+    with pytest.raises(ValueError) as error:
+        matmul.matmul_manager.enable_online_dynamic_quant(model, QuantLayerConfig(), dtype="mxfp4")
+    assert "1.1 (" in str(error.value.__cause__)
+
+
+def test_installer_excludes_what_does_not_fit():
+    model = nn.Sequential(nn.Linear(96, 24), nn.ReLU())
+    config = QuantLayerConfig(exclude_patterns=["0"])
+    assert matmul.enable_weight_quant_linear(model, config, dtype="mxfp4") is model and type(model[0]) is nn.Linear

@@ -33,6 +33,7 @@ from ..ops import xops
 from .mxfp4 import MXFP4Linear
 
 LOG = logging.getLogger(__name__)
+_CAST_WEIGHTS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def dynamic_quant(x: torch.Tensor):
@@ -120,15 +121,20 @@ def enable_weight_quant_linear(model: nn.Module, quant_config: QuantLayerConfig,
     was released are skipped; LoRA '.base_layer' suffixes are undone in the
     replacement name.  dtype 'w8a8' (the reference's transformer path builds the
     W8A8 module for every CLI value, matmul.py:183) or 'mxfp4': MXFP4Linear modules,
-    4-bit weights and activations, which take float32 inputs as BF16 too.
+    4-bit weights and activations, which take float32 inputs as BF16 too.  With 'mxfp4', layers whose
+    shape or type has no 4-bit form are a ValueError that names them all, before any is replaced.
     """
     if dtype not in ('w8a8', 'mxfp4'):
         raise ValueError("xgen_amd provides 'w8a8' and 'mxfp4' modules")
-    for name, layer in list(model.named_modules()):
-        if not quant_config.should_quantize(name, layer):
-            continue
-        if getattr(layer, 'weight', None) is None:
-            continue
+    selected = [(name, layer) for name, layer in model.named_modules()
+                if quant_config.should_quantize(name, layer) and getattr(layer, 'weight', None) is not None]
+    if dtype == 'mxfp4':
+        unfit = [f"{name} {tuple(layer.weight.shape)} {layer.weight.dtype}" for name, layer in selected
+                 if not MXFP4Linear.fits(layer.weight.shape) or layer.weight.dtype not in _CAST_WEIGHTS]
+        if unfit:
+            raise ValueError("MXFP4Linear takes BF16/F16/F32 weights [N, K] with N a multiple of 16 and K of 32; "
+                             f"exclude in the quantization config: {', '.join(unfit)}")
+    for name, layer in selected:
         clean_name = name.replace(".base_layer", "")
         bias = layer.bias.data if getattr(layer, 'bias', None) is not None else None
         if dtype == 'mxfp4':

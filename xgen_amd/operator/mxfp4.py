@@ -112,7 +112,7 @@ class MXFP4Linear(nn.Module):
 
     def __init__(self, weight, bias=None, *, activation=None, weight_rounding="ceil", rounding="ceil", cast_float32=False):
         super().__init__()
-        if weight.ndim != 2 or weight.shape[0] % 16 or weight.shape[1] % 32:
+        if not self.fits(weight.shape):
             raise ValueError("MXFP4Linear requires [N, K] with N a multiple of 16 and K of 32")
         packed, scales = quantize_mxfp4(_device_weight(weight), rounding=weight_rounding)
         self._keep(packed.to(weight.device), scales.to(weight.device), bias, activation, rounding, cast_float32)
@@ -128,6 +128,11 @@ class MXFP4Linear(nn.Module):
         self.register_buffer("weight_scales", scales)
         self.register_buffer("bias", bias.detach().clone() if bias is not None else None)
         self.activation, self.rounding, self.cast_float32 = activation, rounding, bool(cast_float32)
+
+    @staticmethod
+    def fits(shape):
+        """Whether a weight of this shape has a 4-bit form."""
+        return len(shape) == 2 and shape[0] > 0 and shape[1] > 0 and shape[0] % 16 == 0 and shape[1] % 32 == 0
 
     @classmethod
     def from_packed(cls, weight, scales, bias=None, *, activation=None, rounding="ceil", cast_float32=False):
