@@ -45,3 +45,14 @@ def test_installer_excludes_what_does_not_fit():
     model = nn.Sequential(nn.Linear(96, 24), nn.ReLU())
     config = QuantLayerConfig(exclude_patterns=["0"])
     assert matmul.enable_weight_quant_linear(model, config, dtype="mxfp4") is model and type(model[0]) is nn.Linear
+
+
+@pytest.mark.parametrize("dtype", ["w8a8", "mxfp4"])
+def test_the_installer_logs_what_it_installs(dtype, caplog):
+    with caplog.at_level("INFO", logger=matmul.LOG.name):
+        matmul.matmul_manager.enable_online_dynamic_quant(nn.Sequential(nn.ReLU()), QuantLayerConfig(), dtype=dtype)
+        with pytest.raises(ValueError):
+            matmul.matmul_manager.enable_online_dynamic_quant(nn.Sequential(nn.Linear(48, 24, dtype=torch.float64)), QuantLayerConfig(), dtype=dtype)
+    said = [r.getMessage() for r in caplog.records]
+    assert len(said) == 4 and all(dtype.upper() in m for m in said), said
+    assert "installed" in said[1] and "failed" in said[3]

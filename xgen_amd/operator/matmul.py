@@ -166,8 +166,8 @@ class MatmulManager:
 
     def enable_online_dynamic_quant(self, transformer, quant_config: QuantLayerConfig | None = None,
                                     dtype: str = 'w8a8'):
-        """Swap the selected nn.Linear layers of `transformer` for WeightQuantLinearModule in place
-        and return it.  quant_config None: the model's own rule set, chosen from its class
+        """Swap the selected nn.Linear layers of `transformer` for WeightQuantLinearModule (dtype 'mxfp4':
+        MXFP4Linear) in place and return it.  quant_config None: the model's own rule set, chosen from its class
         (xgen_amd.config.detect_config_name).  As in the reference, any failure surfaces as
         ValueError (the cause chained) after being logged."""
         rank = _rank()
@@ -176,15 +176,15 @@ class MatmulManager:
                 name = detect_config_name(transformer)
                 quant_config = get_config(name)
                 LOG.info("rank %d: quant config %r detected for %s", rank, name, type(transformer).__name__)
-            LOG.info("rank %d: replacing linears by W8A8 modules", rank)
+            LOG.info("rank %d: replacing linears by %s modules", rank, str(dtype).upper())
             model = enable_weight_quant_linear(transformer, quant_config, dtype=dtype)
             gc.collect()
             if torch.cuda.is_available():
                 torch.cuda.empty_cache()
         except Exception as error:
-            LOG.error("W8A8 installation failed: %s", error)
+            LOG.error("%s installation failed: %s", str(dtype).upper(), error)
             raise ValueError("Dynamic weight modify model failed. Please try running the program again.") from error
-        LOG.info("rank %d: W8A8 linears installed", rank)
+        LOG.info("rank %d: %s linears installed", rank, str(dtype).upper())
         return model
 
     def enable_vae_conv3d_quant(self, vae):
