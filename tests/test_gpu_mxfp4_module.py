@@ -28,3 +28,17 @@ def test_installed_in_a_float32_model(cuda):
     res, gate, idx = gated_inputs(torch.Generator().manual_seed(3), cuda, 5, 96, 4, 5)
     res = res[None]
     assert torch.equal(model[0].forward_gate_residual(x[None], res, gate, idx), model[0].forward_gate_residual(x[None].to(BF), res, gate, idx))
+
+
+@pytest.mark.parametrize("rounding", [None, "floor", "ceil"])
+def test_shared_rows(cuda, rounding):
+    """Rows that a module quantized give its own result through it and through every other of its rounding."""
+    g = torch.Generator().manual_seed(4)
+    kw = {} if rounding is None else {"rounding": rounding}
+    up, gate = (MXFP4Linear((torch.randn((96, 160), generator=g) * 0.02).to(BF).to(cuda), activation=a, **kw) for a in ("gelu_tanh", None))
+    x = torch.randn((2, 70, 160), generator=g).to(BF).to(cuda)
+    shared = up.quantize_input(x)
+    for linear in (up, gate):
+        assert torch.equal(linear.forward_quantized(*shared), linear(x))
+    other = quantize_mxfp4(x, rounding="floor" if rounding != "floor" else "ceil")
+    assert not torch.equal(up.forward_quantized(*other), up(x))

@@ -159,7 +159,8 @@ class MXFP4Linear(nn.Module):
         return self.forward_quantized(*self.quantize_input(x), out_dtype=x.dtype)
 
     def forward_quantized(self, codes, scales, out_dtype=torch.bfloat16):
-        """The product of rows that are quantized already (several projections of one input)."""
+        """The product of rows that are quantized already (several projections of one input): forward's result for
+        quantize_input's rows; quantize_mxfp4's default rounds the scales otherwise than a module's."""
         return mxfp4_matmul(codes, scales, self.weight, self.weight_scales, bias=self.bias, out_dtype=out_dtype,
                             activation=self.activation)
 
