@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import concurrent.futures
 import os
+import re
 import shutil
 import subprocess
 from pathlib import Path
@@ -35,6 +36,11 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 
+# Sources whose asm statements hold values in accumulator registers by name, from one statement to the next.  The compiler
+# is not aware of that: were it to use one of them itself (a spill), sums would be wrong without an error.
+NAMED_ACCUMULATORS = frozenset({"mxfp4_gemm"})
+_ACCUMULATOR = re.compile(r"(?<![\w.$@])a(?:\d+\b|\[)")
+
 
 def hipcc() -> str:
     path = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
@@ -43,12 +49,43 @@ def hipcc() -> str:
     return path
 
 
-def _compile(src: Path) -> Path:
-    obj = OBJ_DIR / (src.stem + ".o")
-    cmd = [hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src), "-o", str(obj)]
+def _hipcc(src: Path, *args: str) -> None:
+    cmd = [hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", str(src), *args]
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{proc.stdout}")
+
+
+def foreign_accumulators(assembly: str) -> list[str]:
+    """The instructions of gfx950 assembly, other than matrix products and reads of accumulators, that name an accumulator
+    register, and those that use scratch memory."""
+    found = []
+    for line in assembly.splitlines():
+        code = line.split(";")[0].strip()
+        if not code or code.startswith(".") or code.endswith(":"):
+            continue
+        name, _, operands = code.partition(" ") if " " in code else code.partition("\t")
+        if name.startswith("scratch_") or (_ACCUMULATOR.search(operands) and not name.startswith(("v_mfma_", "v_accvgpr_read"))):
+            found.append(code)
+    return found
+
+
+def _check_accumulators(src: Path) -> None:
+    """Raises if the compiler uses accumulator registers, or spills, in a source whose statements hold values in them."""
+    assembly = OBJ_DIR / (src.stem + ".s")
+    _hipcc(src, "--cuda-device-only", "-S", "-o", str(assembly))
+    text = assembly.read_text()
+    found = foreign_accumulators(text)
+    if found or "v_mfma_" not in text:
+        raise RuntimeError(f"{src.name}: the compiler uses accumulator registers or scratch that the kernels' statements "
+                           f"hold values in: {found[:8]}")
+
+
+def _compile(src: Path) -> Path:
+    obj = OBJ_DIR / (src.stem + ".o")
+    _hipcc(src, "-c", "-o", str(obj))
+    if src.stem in NAMED_ACCUMULATORS:
+        _check_accumulators(src)
     return obj
 
 

@@ -73,7 +73,9 @@ XGEN_DMA_AT(3)
 
 // --- the accumulators: fragment (i, j) of a wave's block, weights i and activations j, is AGPRs 16 (4 i + j) .. + 15, all
 // 256 of them, by name.  As variables, the compiler moves some of them where the epilogue joins the loop, right behind
-// the instructions that write them; the rest of the kernel fits the VGPRs, so it has no use for AGPRs of its own.
+// the instructions that write them; the rest of the kernel fits the VGPRs, so it has no use for AGPRs of its own.  The compiler does
+// not know that they hold values between two statements: the build reads this file's assembly, and fails where an
+// instruction other than these statements' names one, or scratch is used.
 constexpr int acc_reg(int i, int j) { return 16 * (F * i + j); }
 
 #define XGEN_MX4(ADDEND, OPSEL) \
@@ -96,7 +98,7 @@ __device__ __forceinline__ float read_acc() {
   asm volatile("v_accvgpr_read_b32 %0, a[%1]" : "=v"(v) : "n"(R));
   return v;
 }
-// Tells the compiler that all of them are taken.
+// Counts all of them in the kernel's registers (it keeps the compiler off them at this place alone).
 __device__ __forceinline__ void take_accumulators() {
 #define XGEN_A(N) "a" #N
 #define XGEN_A10(T) XGEN_A(T##0), XGEN_A(T##1), XGEN_A(T##2), XGEN_A(T##3), XGEN_A(T##4), XGEN_A(T##5), XGEN_A(T##6), XGEN_A(T##7), XGEN_A(T##8), XGEN_A(T##9)
