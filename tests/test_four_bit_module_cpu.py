@@ -3,6 +3,9 @@ import pytest
 import torch
 from torch import nn
 
+from test_experts_cpu import call
+from test_four_bit_cpu import MM
+from xgen_amd import _native as N
 from xgen_amd.config import QuantLayerConfig
 from xgen_amd.operator import matmul, mxfp4
 
@@ -56,3 +59,10 @@ def test_the_installer_logs_what_it_installs(dtype, caplog):
     said = [r.getMessage() for r in caplog.records]
     assert len(said) == 4 and all(dtype.upper() in m for m in said), said
     assert "installed" in said[1] and "failed" in said[3]
+
+
+def test_longest_sequence_of_a_gated_product(built_library):
+    L = N.lib()
+    rows = 1 << 28
+    assert call("xgen_mxfp4_matmul", MM, M=rows, seq=rows, ab=rows * 8)(L) == N.ERR_UNSUPPORTED
+    assert b"2^28" in L.xgen_last_error()

@@ -605,12 +605,14 @@ struct GateParams {  // the gated residual epilogue's inputs (null residual: pla
   int64_t gate_stride = 0, gate_rows = 0;
   const int64_t *indices = nullptr;
   int64_t seq = 0;
+  // MXFP4: this is a chunk of a call's rows, and row 0's place in its sequence (the 8-bit kernels' chunks are whole sequences)
+  bool chunk = false;
+  int64_t first = 0;
 };
 
 struct BlockScales {  // the MXFP4 kind's scale bytes (xgen_mxfp4_quantize's layout) in place of sa and sw
   const uint8_t *x = nullptr;
   int64_t x_block = 0;  // bytes between the blocks of 256 values
-  int64_t x_rows = 0;   // rows of a block from x on: a multiple of two for the whole call, not for each chunk of it
   const uint8_t *w = nullptr;
   int64_t w_block = 0;
 };
@@ -650,11 +652,13 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
     return fail(XGEN_ERR_UNSUPPORTED, "%s: scale, bias and accumulator buffers must be 16-byte aligned", fn);
   if (gated) {
     if (!gp.gate || !gp.indices) return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
-    if (gp.seq <= 0 || M % gp.seq || gp.gate_rows <= 0 || gp.ld_residual < N || gp.gate_stride < N)
+    if (gp.seq <= 0 || (!gp.chunk && M % gp.seq) || gp.gate_rows <= 0 || gp.ld_residual < N || gp.gate_stride < N)
       return fail(XGEN_ERR_INVALID_ARGUMENT, "%s: bad gated residual shape (M %% seq, gate rows, strides)", fn);
     if (gp.ld_residual % 8 || gp.gate_stride % 8 || !aligned16(gp.residual) || !aligned16(gp.gate))
       return fail(XGEN_ERR_UNSUPPORTED, "%s: residual and gate rows must be 16-byte aligned", fn);
     if (M >= 0x7fffffffLL) return fail(XGEN_ERR_UNSUPPORTED, "%s: too many rows", fn);
+    // (32-bit offsets of the indices; the 8-bit kinds' sequences are shorter, as each is in one chunk)
+    if (gp.seq >= (1ll << 28)) return fail(XGEN_ERR_UNSUPPORTED, "%s: a sequence of 2^28 rows or more", fn);
     // 32-bit offsets of the gate rows
     if ((uint64_t)gp.gate_rows * (uint64_t)gp.gate_stride * 2 >= (1ull << 31))
       return fail(XGEN_ERR_UNSUPPORTED, "%s: gate table above 2 GiB", fn);
@@ -672,14 +676,18 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   if (gated) cap(0x7fffffffLL / (2 * gp.ld_residual) - 256);  // residual rows past M below 2^31
   if (rows < M) {
     rows = rows / 256 * 256;                           // whole tile-rows
-    if (gated) rows = rows / gp.seq * gp.seq;          // chunks start at token position 0
+    if (gated && !kMx) rows = rows / gp.seq * gp.seq;  // chunks start at token position 0
     if (rows <= 0) return fail(XGEN_ERR_UNSUPPORTED, "%s: operand rows too long for 32-bit offsets", fn);
     for (int64_t m0 = 0; m0 < M; m0 += rows) {
       const int64_t mi = M - m0 < rows ? M - m0 : rows;
       GateParams gc = gp;
-      if (gated) gc.residual = static_cast<const uint8_t *>(gp.residual) + m0 * gp.ld_residual * 2;
+      if (gated) {
+        gc.residual = static_cast<const uint8_t *>(gp.residual) + m0 * gp.ld_residual * 2;
+        gc.chunk = kMx;
+        gc.first = kMx ? m0 % gp.seq : 0;
+      }
       BlockScales bc = bs;
-      if (kMx) bc.x = bs.x + m0 * 8, bc.x_rows = bs.x_rows - m0;
+      if (kMx) bc.x = bs.x + m0 * 8;  // (an even row: the scales' rows behind a chunk's are pairs too)
       const int st = gemm_entry<KIND>(
           fn, static_cast<const uint8_t *>(a) + m0 * lda, lda, w, ldw, mi, N, K, sa_stride ? sa + m0 : sa, sa_stride,
           sw, sw_stride, bias, bias_dtype, activation, static_cast<uint8_t *>(out) + m0 * ldo * 2, out_dtype, ldo,
@@ -732,7 +740,8 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   g.gate_rows = gp.gate_rows;
   g.indices = gp.indices;
   g.seq = (uint32_t)gp.seq;
-  g.seq_magic = g.seq_shift = g.seq_first = 0;  // (read by the gated kernels only)
+  g.seq_magic = g.seq_shift = 0;  // (read by the gated kernels only)
+  g.seq_first = (uint32_t)gp.first;
   if (gated) {
     const FastDiv fd = make_fastdiv((uint32_t)gp.seq);
     g.seq_magic = fd.m;
@@ -744,8 +753,7 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
   g.ws = bs.w;
   g.xs_block = bs.x_block;
   g.ws_block = bs.w_block;
-  // (below 2^31: M rows of at least 16 bytes are; a last chunk that starts at an odd row has no row behind its own)
-  g.xs_rows = (uint32_t)((M % 2 && M < bs.x_rows ? M + 1 : M) * 8);
+  g.xs_rows = (uint32_t)((M + M % 2) * 8);  // (below 2^31: M rows of at least 16 bytes are)
   g.ws_rows = (uint32_t)(N * 8);
   g.kt4 = (int)(((K + BK - 1) / BK + 3) / 4 * 4);
   const int64_t out_bytes = ((M - 1) * ldo + N) * 2;
@@ -772,13 +780,13 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
       r.a += m0 * lda;
       r.a_bytes = (uint32_t)((m - 1) * lda + K);
       r.xs += m0 * 8;
-      r.xs_rows = (uint32_t)((m % 2 && m0 + m < bs.x_rows ? m + 1 : m) * 8);
+      r.xs_rows = (uint32_t)((m + m % 2) * 8);
       r.out = static_cast<uint8_t *>(out) + m0 * ldo * 2;
       r.out_bytes = (uint32_t)(((m - 1) * ldo + N) * 2);
       if (gated) {
         r.residual += m0 * gp.ld_residual * 2;
         r.residual_bytes = (uint32_t)(((m - 1) * gp.ld_residual + N) * 2);
-        r.seq_first = (uint32_t)(m0 % gp.seq);
+        r.seq_first = (uint32_t)((gp.first + m0) % gp.seq);
       }
       return r;
     };
@@ -902,7 +910,6 @@ extern "C" int xgen_mxfp4_matmul(const void *a, int64_t lda, const void *a_scale
   BlockScales bs;
   bs.x = static_cast<const uint8_t *>(a_scales);
   bs.x_block = a_block_stride;
-  bs.x_rows = M + M % 2;
   bs.w = static_cast<const uint8_t *>(w_scales);
   bs.w_block = w_block_stride;
   return gemm_entry<kMx4>(fn, a, lda, w, ldw, M, N, K / 2, nullptr, 0, nullptr, 0, bias, bias_dtype, activation, out,
