@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import xgen_amd  # noqa: F401
-from xgen_amd.operator.mxfp4 import mxfp4_matmul, pack_scales
+from xgen_amd.operator.mxfp4 import dequantize_mxfp4, mxfp4_matmul, pack_scales, quantize_mxfp4
 
 pytestmark = pytest.mark.gpu
 BF, U8 = torch.bfloat16, torch.uint8
@@ -26,3 +26,22 @@ def test_gated_sequences_past_one_launch(cuda, m, seq):
         at = torch.arange(first, last, device=cuda) % seq
         part = mxfp4_matmul(a[0][first:last], pack_scales(sa[first:last]), *w, residual=res[first:last], gate_table=gate, indices=idx[at])
         assert torch.equal(out[first:last], part), first
+
+
+def test_rows_past_one_launch(cuda):
+    """More rows than a launch's threads: the last ones, and those at every launch's border, as calls of their own give them."""
+    r, k, launch = (1 << 28) + 49, 32, 1 << 27
+    base = torch.randn((1 << 20, k), generator=torch.Generator(device=cuda).manual_seed(1), device=cuda).to(BF)
+    x = torch.empty((r, k), dtype=BF, device=cuda)
+    for first in range(0, r, len(base)):
+        x[first:first + len(base)] = base[:r - first]
+    codes, scales = quantize_mxfp4(x)
+    back = dequantize_mxfp4(codes, scales)
+    assert scales.shape == (1, r + 1, 8) and not scales[0, r].any()
+    for first in (0, launch - 40, 2 * launch - 40, r - 49):
+        last = min(r, first + 80)
+        want = quantize_mxfp4(x[first:last])
+        assert torch.equal(codes[first:last], want[0]) and torch.equal(scales[0, first:last], want[1][0, :last - first]), first
+        assert torch.equal(back[first:last], dequantize_mxfp4(*want)), first
+    period = codes[:len(base)]
+    assert all(torch.equal(codes[f:f + len(base)], period[:r - f]) for f in range(0, r, 16 * len(base)))

@@ -23,6 +23,8 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kCols = 512;                    // values of a row that a wave takes at once: 8 per lane
 constexpr int kRows = 4;                      // rows a wave takes: that many loads in flight per lane
 constexpr int kTileRows = kWaves * kRows;     // a workgroup's rows: their scale bytes fill whole lines
+// rows of a launch: a grid's threads are counted in 32 bits
+constexpr int64_t kLaunchRows = (int64_t)kTileRows * ((1ll << 32) / kThreads / 2);
 
 struct RowsArgs {
   const uint8_t *x;       // values, or codes (dequantize)
@@ -150,8 +152,17 @@ int check_rows(const char *fn, int64_t rows, int64_t K, const void *dense, int64
   return XGEN_OK;
 }
 
-dim3 rows_grid(const RowsArgs &p) {
-  return dim3((unsigned)((p.rows + kTileRows - 1) / kTileRows), (unsigned)(((int64_t)p.K + kCols - 1) / kCols));
+// launch(args, grid) for the rows of each launch (whole workgroups, so that the scales' last row stays the last launch's)
+template <class Launch>
+void each_launch(const RowsArgs &p, Launch launch) {
+  for (int64_t first = 0; first < p.rows; first += kLaunchRows) {
+    RowsArgs q = p;
+    q.x += first * p.ldx;
+    q.out += first * p.ldo;
+    q.scales += first * 8;
+    q.rows = p.rows - first < kLaunchRows ? p.rows - first : kLaunchRows;
+    launch(q, dim3((unsigned)((q.rows + kTileRows - 1) / kTileRows), (unsigned)(((int64_t)p.K + kCols - 1) / kCols)));
+  }
 }
 
 }  // namespace
@@ -172,8 +183,10 @@ extern "C" int xgen_mxfp4_quantize(int in_dtype, const void *x, int64_t rows, in
   const RowsArgs p = {static_cast<const uint8_t *>(x), ldx * 2, rows, (int)K, (int)((K + 255) / 256),
                       static_cast<uint8_t *>(codes), ld_codes, static_cast<uint8_t *>(scales), block_stride,
                       rounding == XGEN_MX_CEIL};
-  if (in_dtype == XGEN_DTYPE_BF16) quantize_kernel<XGEN_DTYPE_BF16><<<rows_grid(p), kThreads, 0, stream>>>(p);
-  else quantize_kernel<XGEN_DTYPE_F16><<<rows_grid(p), kThreads, 0, stream>>>(p);
+  each_launch(p, [&](const RowsArgs &q, dim3 grid) {
+    if (in_dtype == XGEN_DTYPE_BF16) quantize_kernel<XGEN_DTYPE_BF16><<<grid, kThreads, 0, stream>>>(q);
+    else quantize_kernel<XGEN_DTYPE_F16><<<grid, kThreads, 0, stream>>>(q);
+  });
   return launch_status(fn);
 }
 
@@ -189,8 +202,10 @@ extern "C" int xgen_mxfp4_dequantize(const void *codes, int64_t ld_codes, const 
   const RowsArgs p = {static_cast<const uint8_t *>(codes), ld_codes, rows, (int)K, (int)((K + 255) / 256),
                       static_cast<uint8_t *>(out), ldo * size, static_cast<uint8_t *>(const_cast<void *>(scales)),
                       block_stride, 0};
-  if (out_dtype == XGEN_DTYPE_BF16) dequantize_kernel<XGEN_DTYPE_BF16><<<rows_grid(p), kThreads, 0, stream>>>(p);
-  else if (out_dtype == XGEN_DTYPE_F16) dequantize_kernel<XGEN_DTYPE_F16><<<rows_grid(p), kThreads, 0, stream>>>(p);
-  else dequantize_kernel<XGEN_DTYPE_F32><<<rows_grid(p), kThreads, 0, stream>>>(p);
+  each_launch(p, [&](const RowsArgs &q, dim3 grid) {
+    if (out_dtype == XGEN_DTYPE_BF16) dequantize_kernel<XGEN_DTYPE_BF16><<<grid, kThreads, 0, stream>>>(q);
+    else if (out_dtype == XGEN_DTYPE_F16) dequantize_kernel<XGEN_DTYPE_F16><<<grid, kThreads, 0, stream>>>(q);
+    else dequantize_kernel<XGEN_DTYPE_F32><<<grid, kThreads, 0, stream>>>(q);
+  });
   return launch_status(fn);
 }
