@@ -47,9 +47,9 @@ struct Heads {
 
 struct RotateArgs {
   Heads t[2];          // queries, keys
-  int64_t tokens;
+  uint32_t first, end; // the tokens of this launch
   FastDiv seq;         // token t = b * seq + s
-  FastDiv waves;       // wave i = token * waves + part: GROUPS groups of 64 / LANES heads
+  FastDiv waves;       // wave i = (token - first) * waves + part: GROUPS groups of 64 / LANES heads
   int query_waves;     // the parts that are queries'
   int dim, pairs;
   int norm, weight_dtype;
@@ -103,10 +103,10 @@ template <int DT, int LANES, int PAIRING, int GROUPS, bool PAST>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs p) {
   const int lane = threadIdx.x & 63;
   const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + (threadIdx.x >> 6)));
-  const uint32_t token = fast_div(id, p.waves);
-  if (token >= p.tokens) return;
+  const uint32_t nth = fast_div(id, p.waves), token = p.first + nth;
+  if (token >= p.end) return;
   // (queries' waves first: a wave's groups are of one set)
-  const int part = (int)(id - token * p.waves.d);
+  const int part = (int)(id - nth * p.waves.d);
   const bool keys = part >= p.query_waves;
   const Heads &t = p.t[keys];
   const uint32_t b = fast_div(token, p.seq), s = token - b * p.seq.d;
@@ -357,21 +357,19 @@ extern "C" int xgen_qk_norm_rope(int dtype, const void *q, int64_t q_stride_batc
   if ((q_heads && (q_stride_batch % 8 || q_stride_seq % 8 || q_stride_head % 8)) ||
       (k_heads && (k_stride_batch % 8 || k_stride_seq % 8 || k_stride_head % 8)))
     return fail(XGEN_ERR_UNSUPPORTED, "%s: strides must be multiples of 8", fn);
+  if (q_heads >= (1 << 24) || k_heads >= (1 << 24) || batch >= (1ll << 31) || seq >= (1ll << 31) || batch * seq >= (1ll << 31))
+    return fail(XGEN_ERR_UNSUPPORTED, "%s: too many tokens or heads", fn);
   int lanes = 2;
   while (lanes * 8 < dim) lanes *= 2;
   const int64_t per = 64 / lanes, groups_q = (q_heads + per - 1) / per, groups_k = (k_heads + per - 1) / per;
   const bool past = batch * seq * (q_heads + k_heads) * dim * 4 > kLastLevelCacheBytes;  // read and written
   const int groups = past ? 4 : batch * seq * (groups_q + groups_k) <= kFewGroups ? 1 : 2;
   const int64_t waves_q = (groups_q + groups - 1) / groups, waves = waves_q + (groups_k + groups - 1) / groups;
-  if (q_heads >= (1 << 24) || k_heads >= (1 << 24) || batch >= (1ll << 31) || seq >= (1ll << 31) ||
-      batch * seq >= (1ll << 31) || batch * seq * waves >= (1ll << 31) - kWaves)
-    return fail(XGEN_ERR_UNSUPPORTED, "%s: too many tokens or heads", fn);
   RotateArgs p;
   p.t[0] = {static_cast<const uint8_t *>(q), q_stride_batch * 2, q_stride_seq * 2, q_stride_head * 2, q_weight,
             static_cast<uint8_t *>(q_out), (int)q_heads};
   p.t[1] = {static_cast<const uint8_t *>(k), k_stride_batch * 2, k_stride_seq * 2, k_stride_head * 2, k_weight,
             static_cast<uint8_t *>(k_out), (int)k_heads};
-  p.tokens = batch * seq;
   p.seq = make_fastdiv((uint32_t)seq);
   p.waves = make_fastdiv((uint32_t)waves);
   p.query_waves = (int)waves_q;
@@ -387,9 +385,16 @@ extern "C" int xgen_qk_norm_rope(int dtype, const void *q, int64_t q_stride_batc
   p.positions = positions;
   p.position_batch = position_stride_batch;
   const int pairing = interleaved ? kBeside : pairs % 8 == 0 ? kHalves : kHalvesAny;
-  const unsigned blocks = (unsigned)((batch * seq * waves + kWaves - 1) / kWaves);
-  if (dtype == XGEN_DTYPE_BF16) launch_rotate<XGEN_DTYPE_BF16>(p, lanes, pairing, groups, past, blocks, stream);
-  else launch_rotate<XGEN_DTYPE_F16>(p, lanes, pairing, groups, past, blocks, stream);
+  // (a grid's threads are counted in 32 bits; waves is 2^25 at most)
+  const int64_t tokens = batch * seq, step = (1ll << 25) / waves;
+  for (int64_t first = 0; first < tokens; first += step) {
+    const int64_t end = tokens - first < step ? tokens : first + step;
+    p.first = (uint32_t)first;
+    p.end = (uint32_t)end;
+    const unsigned blocks = (unsigned)(((end - first) * waves + kWaves - 1) / kWaves);
+    if (dtype == XGEN_DTYPE_BF16) launch_rotate<XGEN_DTYPE_BF16>(p, lanes, pairing, groups, past, blocks, stream);
+    else launch_rotate<XGEN_DTYPE_F16>(p, lanes, pairing, groups, past, blocks, stream);
+  }
   return launch_status(fn);
 }
 
