@@ -222,8 +222,13 @@ int quantize_rows_typed(const void *x, int64_t rows, int64_t cols, int64_t ldx, 
   } else if (vec && cols <= 2048 * 8) {
     launch_vec<DT, OUT, ACT, 4, 8>(x, rows, cols, ldx, q, ldq, scale, stream);
   } else {
-    quant_rows_generic_kernel<DT, OUT, ACT><<<dim3((unsigned)rows), dim3(kThreads), 0, stream>>>(
-        static_cast<const uint16_t *>(x), rows, cols, ldx, static_cast<uint8_t *>(q), ldq, scale);
+    constexpr int64_t kLaunchRows = (1ll << 32) / kThreads / 2;  // (a grid's threads are counted in 32 bits)
+    for (int64_t first = 0; first < rows; first += kLaunchRows) {
+      const int64_t n = rows - first < kLaunchRows ? rows - first : kLaunchRows;
+      quant_rows_generic_kernel<DT, OUT, ACT><<<dim3((unsigned)n), dim3(kThreads), 0, stream>>>(
+          static_cast<const uint16_t *>(x) + first * ldx, n, cols, ldx, static_cast<uint8_t *>(q) + first * ldq, ldq,
+          scale + first);
+    }
   }
   return XGEN_OK;
 }
