@@ -80,7 +80,7 @@ def rotary_frequencies(dim, *, base=10000.0, scaling=None, factor=1.0, trained_l
         return f / factor, 1.0
     if scaling not in ("bands", "ramp"):
         raise ValueError("scaling must be None, 'linear', 'base', 'bands' or 'ramp'")
-    if trained_length is None or not 0 < low < high:
+    if trained_length is None or not trained_length > 0 or not 0 < low < high:
         raise ValueError(f"rotary_frequencies: scaling {scaling!r} needs trained_length and 0 < low < high")
     if scaling == "bands":
         kept = ((f * trained_length / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
