@@ -33,7 +33,7 @@ def library_path():
 
 def qk_norm_rope(q, k, cos, sin, *, positions=None, q_weight=None, k_weight=None, norm="rms", eps=1e-6, layout="half"):
     """(q', k') contiguous, of q [B, S, H, D] and k [B, S, Hk, D], BF16/F16 views with any strides (read in place where
-    heads start on 16 bytes, copied otherwise); D a multiple of 8 up to 512.  `norm` "rms", "layer" or None over each
+    heads start on 16 bytes, copied otherwise); D a multiple of 8 up to 512.  `norm` "rms", "layer" (without a bias) or None over each
     head, with weights BF16/F16/F32 [D] or None.  cos, sin float32 [P, R/2]; positions int64 [S] or [B, S] into them, None
     for 0 .. S - 1; a position outside makes its token's heads NaN.  Arithmetic is fp32, rounded once."""
     if q.requires_grad or k.requires_grad or any(t is not None and t.requires_grad for t in (q_weight, k_weight, cos, sin)):
@@ -59,10 +59,13 @@ def rotary_frequencies(dim, *, base=10000.0, scaling=None, factor=1.0, trained_l
       None       as they are
       "linear"   all divided by factor (positions interpolated)
       "base"     the base raised to base * factor^(dim / (dim - 2)): the slowest pair as "linear", the fastest as it is
+                 (NTK-aware scaling)
       "bands"    by turns over trained_length, t = frequency * trained_length / (2 pi): pairs of `high` turns or more
                  as they are, of `low` or fewer divided by factor, between them blended in proportion to t
+                 (configurations' rope type "llama3"; they give low_freq_factor and high_freq_factor, 1 and 4)
       "ramp"     as "bands", but blended in proportion to the pair's place between those of `high` and `low` turns,
                  and the table scaled by 0.1 ln(factor) + 1 (attention logits grow by its square)
+                 (YaRN, with its whole-pair ends and its guard of 0.001; beta_fast is high, beta_slow low)
     """
     if dim <= 0 or dim % 2:
         raise ValueError("rotary_frequencies: an even dim required")
