@@ -576,7 +576,8 @@ int xgen_mxfp4_dequantize(const void *codes, int64_t ld_codes, const void *scale
  * for the blocks past K included.  A row or weight row with a scale of 255 gives NaN.  bias: NULL or [N] of BF16, F16 or F32.  residual NULL or BF16
  * [M, N]; gate_table BF16 [gate_rows, N] with indices int64 [seq], M a multiple of seq (an index outside: a NaN row).
  * K a multiple of 32, N of 16; rows, bias and scale blocks 16-byte aligned; w below 2 GiB; seq below 2^28.  M is
- * not bounded by 32-bit offsets, as xgen_scaled_mm_fp8's, nor is seq.  out overlaps no operand.
+ * not bounded by 32-bit offsets, as xgen_scaled_mm_fp8's, nor is seq (but 256 rows of each operand are: up to 1 GiB).  out
+ * overlaps no operand.
  */
 int xgen_mxfp4_matmul(const void *a, int64_t lda, const void *a_scales, int64_t a_block_stride, const void *w,
                       int64_t ldw, const void *w_scales, int64_t w_block_stride, int64_t M, int64_t N, int64_t K,

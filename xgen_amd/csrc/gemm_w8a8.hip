@@ -660,8 +660,14 @@ int gemm_entry(const char *fn, const void *a, int64_t lda, const void *w, int64_
     // (32-bit offsets of the indices; the 8-bit kinds' sequences are shorter, as each is in one chunk)
     if (gp.seq >= (1ll << 28)) return fail(XGEN_ERR_UNSUPPORTED, "%s: a sequence of 2^28 rows or more", fn);
     // 32-bit offsets of the gate rows
-    if ((uint64_t)gp.gate_rows * (uint64_t)gp.gate_stride * 2 >= (1ull << 31))
+    if (gp.gate_rows > 1 && (uint64_t)gp.gate_rows * (uint64_t)gp.gate_stride * 2 >= (1ull << 31))
       return fail(XGEN_ERR_UNSUPPORTED, "%s: gate table above 2 GiB", fn);
+  }
+  if (M == 1 && (lda != K || ldo != N || (gated && gp.ld_residual != N))) {  // (what is between rows says nothing)
+    GateParams gc = gp;
+    gc.ld_residual = N;
+    return gemm_entry<KIND>(fn, a, K, w, ldw, M, N, K, sa, sa_stride, sw, sw_stride, bias, bias_dtype, activation, out,
+                            out_dtype, N, acc_out, stream, gc, bs);
   }
   // The kernels address the activation rows, the output rows and the residual rows through 32-bit
   // buffer offsets (rows past M of the last tile-row included).  A call whose rows pass those

@@ -135,6 +135,16 @@ Tensor kernel_rows(const Tensor &t, int64_t row_align) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// Rows so far apart that a product, which reads them through 32-bit offsets, would take few of them a launch (a position of
+// each of some long sequences): copied.  A single row is taken where it is.
+bool far_apart(const Tensor &t) {
+  return t.size(0) > 1 && t.stride(0) > t.size(1) && t.stride(0) * (int64_t)t.element_size() > (1 << 21);
+}
+Tensor near_rows(const Tensor &t, int64_t row_align) {
+  const Tensor r = kernel_rows(t, row_align);
+  return far_apart(r) ? r.clone(at::MemoryFormat::Contiguous) : r;
+}
+
 // t contiguous with a 16-byte aligned base (copied if not).
 Tensor aligned_flat(const Tensor &t) {
   Tensor c = t.contiguous();
@@ -290,7 +300,7 @@ struct MmOperands {
   int bias_dtype;
   const void *bias_ptr;
   MmOperands(const Tensor &a_in, const Tensor &w_in, const Tensor &sa, const Tensor &sw, const OptTensor &b)
-      : a(kernel_rows(a_in, 16)), w(kernel_rows(w_in, 16)), a_scale(sa.contiguous()), w_scale(sw.contiguous()) {
+      : a(near_rows(a_in, 16)), w(kernel_rows(w_in, 16)), a_scale(sa.contiguous()), w_scale(sw.contiguous()) {
     if (b) bias = b->contiguous();
     sa_stride = a_scale.numel() == a.size(0) && a.size(0) > 1 ? 1 : 0;
     sw_stride = w_scale.numel() == w.size(0) && w.size(0) > 1 ? 1 : 0;
@@ -348,7 +358,7 @@ Tensor scaled_mm_gate_residual(const Tensor &a, const Tensor &w, const Tensor &a
   Tensor out = empty({M, Nf}, at::kBFloat16, a);
   if (M == 0) return out;
   const MmOperands o(a, w, a_scale, w_scale, bias);
-  const Tensor residual = kernel_rows(residual_in, 8), gate = kernel_rows(gate_in, 8), indices = indices_in.contiguous();
+  const Tensor residual = near_rows(residual_in, 8), gate = kernel_rows(gate_in, 8), indices = indices_in.contiguous();
   check(api().xgen_w8a8_gate_residual(
             dtype_code(a.scalar_type()), o.a.data_ptr(), o.a.stride(0), o.w.data_ptr(), o.w.stride(0), M, Nf, K,
             o.a_scale.data_ptr<float>(), o.sa_stride, o.w_scale.data_ptr<float>(), o.sw_stride, o.bias_ptr,
@@ -662,7 +672,7 @@ struct MxRows {
   void lay_out() {
     if (rows == 0) return;
     codes = rows_view(codes);
-    if (!aligned16(codes) || rows_apart(codes) % 16) codes = codes.clone(at::MemoryFormat::Contiguous);
+    if (!aligned16(codes) || rows_apart(codes) % 16 || far_apart(codes)) codes = codes.clone(at::MemoryFormat::Contiguous);
     ld = rows_apart(codes);
     scales = aligned_flat(scales);
     block = (rows + rows % 2) * 8;
@@ -719,7 +729,7 @@ Tensor mxfp4_matmul(const Tensor &a_in, const Tensor &a_scales, const Tensor &w_
   if (M == 0) return out;
   a.lay_out();
   w.lay_out();
-  const Tensor bias = optional_flat(bias_in), residual = gated ? kernel_rows(*residual_in, 8) : Tensor();
+  const Tensor bias = optional_flat(bias_in), residual = gated ? near_rows(*residual_in, 8) : Tensor();
   const Tensor gate = gated ? kernel_rows(*gate_in, 8) : Tensor(), indices = gated ? indices_in->contiguous() : Tensor();
   check(entry(a.codes.data_ptr(), a.ld, a.scales.data_ptr(), a.block, w.codes.data_ptr(), w.ld, w.scales.data_ptr(), w.block,
               M, Nf, a.K, optional_ptr(bias), bias.defined() ? dtype_code(bias.scalar_type()) : XGEN_DTYPE_NONE, (int)activation,
