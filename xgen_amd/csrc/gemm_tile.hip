@@ -63,8 +63,11 @@ constexpr TileCost kTileCosts[4][kTiles + 1] = {
 // stores its accumulators stores three times the bytes, on the 256-row tiles all at the end: 15% for them (at
 // the lines above, 15,624 x 5,376 x 384 exact: 228 us on 256 x 192, 148 on the large kernel, and 44
 // of 1,776 calls more than 3% slower than on it; so 18, most of them under K = 1,024, 17% at most).
-// MXFP4 calls 4% throughout (its figures are from 78 shapes, up to 14,336 x 5,376: the choice is within 0.2% of the
-// best tile on the average; by INT8's figures, with which its kernels began, 1.25%).
+// MXFP4 calls 4% throughout.  Its figures are fitted to 78 plain shapes up to 14,336 x 5,376 (on these the choice is within 0.2%
+// of the best tile on the average; by INT8's figures, with which its kernels began, 1.25%), and gated calls take the same. On 110
+// others (M 2 to 9,000, N 384 to 15,648, K 288 to 13,600) the time is on the average that of the best tile in plain calls, two
+// launches among them (up to 13% below it; without their gains 0.8% above), and 0.3% above in gated ones (1.1%); at most
+// 14% above (4,052 x 5,008 x 320: 28.2 us on 256 x 256, 24.8 on 256 x 192) and 7.5% (3 x 6,256 x 480: 5.2 us, 4.8).
 float keep_large(int kind, int tile, int64_t K, bool gated, bool accumulators) {
   if (kind == kMx4) return 0.96f;
   if (accumulators && kTileSizes[tile].m == 256) return 0.85f;

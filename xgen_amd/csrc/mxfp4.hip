@@ -10,7 +10,8 @@
 // Scale bytes lie as the matrix product's lanes read them (gemm_w8a8.h): [256 values][row][8], block i of a
 // row's 256 values at (i mod 2) * 4 + i / 2, so that 16 rows share a line and a lane's four blocks a dword.
 //
-// Memory bounds both directions: 15,624 x 5,376 of bf16 takes 40 us either way, 5.3 TB/s, as a copy of as many bytes; 2 x 2,048
+// Memory bounds both directions: 15,624 x 5,376 of bf16 takes 40 us either way, 5.3 TB/s, as a copy of as many bytes (to float32
+// 83 us, 4.6 TB/s); 2 x 2,048
 // 2.4 us, a launch and one load's way.  A wave takes 4 rows of 512 values, so that four loads are in flight in each
 // lane, and a workgroup 16 rows, whose scale bytes are whole lines.
 #include "xgen_common.h"

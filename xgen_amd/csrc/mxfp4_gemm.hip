@@ -15,14 +15,17 @@
 //
 // Epilogue: the DMA places the weight rows so that a lane's accumulators are runs of eight consecutive features; they
 // pass through a 4.5 KB area of LDS of the wave's own, 32 tokens of 64 features at a time, so that each row is stored as one
-// 128-byte line (stored from the accumulators' places, 32 bytes of a row at a time, the epilogue took 142 us of
-// the call below).  Past the caches: the output is more than they hold wherever this kernel's tiles fill the card.
+// 128-byte line (stored from the accumulators' places, 32 bytes of a row at a time, the call below took 142 us
+// more).  Past the caches: the output is more than they hold wherever this kernel's tiles fill the card.
 //
-// What bounds it: the matrix units' power.  15,624 x 14,336 x 5,376 takes 532 to 550 us, 4.4 PFLOP/s: 1.69 us a pair and CU
-// on normally distributed values, 1.02 on zeros, with the same instructions; a loop of these MFMAs alone does 6.2 to
-// 6.7 PFLOP/s on random codes, 9.65 on zeros.  GELU there 582 to 600 (its arithmetic stands between the MFMAs of an epilogue).
-// 15,360 x 5,376 x 14,336 and 264 rows more in a launch of their own: 530 us, with the gated residual 587 (its reads are
-// waited for).
+// What bounds it: the matrix units' power.  15,624 x 14,336 x 5,376, back to back, on normally distributed values takes 517 to
+// 550 us, 4.4 to 4.7 PFLOP/s, and twice the K twice that; with zeros in both operands, the same instructions, 423 us (5.7): 341
+// in the loop over K (from twice the K: 1.16 us a pair, 7.1 PFLOP/s) and 82 beside it, 5.9 us a round of tiles for the
+// epilogues and the waits behind them.  On values those cost little, since the power that they leave is the loop's.  A loop of
+// these MFMAs alone does 6.2 to 6.7 PFLOP/s on random codes, 9.65 on zeros.  GELU there 570 to 600 (its arithmetic
+// stands between the MFMAs of an epilogue).  15,360 x 5,376 x 14,336 and 264 rows more in a launch of their own: 493 to 530 us, with
+// the gated residual 574 to 587 (its reads are waited for; that kernel keeps 68 scalars in lanes of vector registers over the
+// loop, the others none).
 //
 // The same on the fragments of 16 x 16 x 128, which draw less power (7.3 PFLOP/s in the loop): 575 us; there are twice
 // as many MFMAs and reads of scales to issue, and the power saved is not what it gained.

@@ -17,7 +17,8 @@
 //
 // Memory bounds it: 15,624 tokens of 112 heads of 128, 904 MB, 172 us (5.2 TB/s, a copy's rate; a wave that took queries and
 // keys in turn and read its weights value by value took 366); 3,910 tokens of 40 heads of 64 11 us; one token of each of 4
-// requests 3.3 us.
+// requests 3.3 us.  Halves whose pairs are no multiple of 8 read every partner by itself: 422 to 488 us at the
+// first of these (10, 60 or 63 pairs; 16, 48 or 64: 166); pairs side by side whose number is none of 4, 162 to 166 (150).
 #include <utility>
 
 #include "fastdiv.h"
@@ -272,7 +273,9 @@ void launch_rotate(const RotateArgs &p, int lanes, int pairing, int groups, bool
 // cos and sin of positions[p, axis[i]] * f[i], times a factor.  The angle is formed and brought into
 // [-pi/4, pi/4] in 64 bits (pi/2 in two parts), where series up to r^13 and r^12 are right to 2^-38 of the value:
 // at position 10^6 a 32-bit angle would be off by 0.03.  One rounding, to fp32.  A value a thread: its chain of 64-bit
-// operations bounds it (15,624 x 64 pairs 5.6 us, 4 x 64 1.7).
+// operations bounds it: 96 vector instructions a wave, 2.4 us of the card's issue for 15,624 x 64 pairs, which take 5.2 us in a
+// graph (a launch of 4 x 64 1.9); the waves wait for the axis and for the position behind it two thirds of their time.  Of
+// 249,984 places, 51 us, the issue is 39.
 // ---------------------------------------------------------------------------
 struct TableArgs {
   const int64_t *positions;
